@@ -43,6 +43,7 @@ class SequenceCache:
         self.pages = IndexAllocator(self.num_pages, "page")
         self.lengths = [0] * max_sequences
         self._owned = [[] for _ in range(max_sequences)]
+        self._holders = {}  # page -> how many sequences hold it, for pages that more than one does
         self._table_host = np.zeros((max_sequences, per_seq), dtype=np.int32)
         self.block_table = torch.zeros((max_sequences, per_seq), dtype=torch.int32, device=self.device)
         self._dirty = {}  # slot -> (first, last+1) columns of the table not yet on the device
@@ -131,12 +132,80 @@ class SequenceCache:
         self.lengths[slot] = new
         return old
 
+    def fork(self, slot: int, count: int = 1, length: int | None = None) -> list:
+        """``count`` new sequences that begin with the first ``length`` tokens of ``slot`` (all of them by default); returns their slots.
+
+        Pages that are full are shared: they are only read from then on, and each goes back when the last
+        sequence that holds it is closed.  The page that is not full is copied for each (on the device, all tensors
+        in one launch), and so is the per-sequence state, which stands behind the last token: with one, only whole
+        sequences fork.  Nothing changes if there are not enough slots or pages."""
+        if not self.slots.is_held(slot):
+            raise ValueError(f"slot {slot} is not open")
+        if count < 1:
+            raise ValueError(f"a fork makes one sequence or more, not {count}")
+        have = self.lengths[slot]
+        length = have if length is None else length
+        if not 0 <= length <= have:
+            raise ValueError(f"slot {slot} holds {have} tokens: none can begin with {length} of them")
+        if self.state and length != have:
+            raise ValueError(f"the state of slot {slot} stands behind all of its {have} tokens, not behind {length}")
+        whole, rest = divmod(length, PAGE_TOKENS)
+        slots = self.slots.take_many(count)
+        try:
+            fresh = self.pages.take_many(count if rest else 0)
+        except CacheFull:
+            for new in reversed(slots):
+                self.slots.give_back(new)
+            raise
+        shared = self._owned[slot][:whole]
+        for page in shared:
+            self._holders[page] = self._holders.get(page, 1) + count
+        for i, new in enumerate(slots):
+            pages = shared + fresh[i:i + 1]
+            self._owned[new] = pages
+            self.lengths[new] = length
+            self._table_host[new, :len(pages)] = pages
+            if pages:
+                self._dirty[new] = (0, len(pages))
+        if fresh:
+            self._copy_items(self.keys + self.values, [self._owned[slot][whole]] * count, fresh, 1)
+        if self.state:
+            self._copy_items(list(self.state.values()), [slot] * count, slots, 0)
+        return slots
+
+    def _copy_items(self, tensors, source, target, dim) -> None:
+        if self.device.type != "cuda":           # (bookkeeping without a device)
+            for t in tensors:
+                t.index_copy_(dim, torch.tensor(target), t.index_select(dim, torch.tensor(source)))
+            return
+        from .. import ops
+
+        ops.cache_copy_pages(tensors, source, target, dim=dim)
+
+    def shorten(self, slot: int, length: int) -> None:
+        """Forget the tokens of ``slot`` behind the first ``length`` (its pages stay with it).  Not into a page that
+        it shares with another sequence, and not with a per-sequence state, which cannot go back."""
+        if not self.slots.is_held(slot):
+            raise ValueError(f"slot {slot} is not open")
+        have = self.lengths[slot]
+        if not 0 <= length <= have:
+            raise ValueError(f"slot {slot} holds {have} tokens: it cannot be shortened to {length}")
+        if self.state and length != have:
+            raise ValueError(f"the state of slot {slot} stands behind all of its {have} tokens")
+        if any(page in self._holders for page in self._owned[slot][length // PAGE_TOKENS:]):
+            raise ValueError(f"slot {slot} shares a page behind its token {length} with another sequence")
+        self.lengths[slot] = length
+
     def close_sequence(self, slot: int) -> None:
-        """Give back the slot and its pages."""
+        """Give back the slot and its pages (those it shares once their last holder is closed)."""
         if not self.slots.is_held(slot):
             raise ValueError(f"slot {slot} is not open, so it cannot be closed")
         for page in self._owned[slot]:
-            self.pages.give_back(page)
+            left = self._holders.pop(page, 1) - 1
+            if left == 0:
+                self.pages.give_back(page)
+            elif left > 1:
+                self._holders[page] = left
         self._owned[slot] = []
         self.lengths[slot] = 0
         self._dirty.pop(slot, None)
@@ -171,19 +240,23 @@ class SequenceCache:
         self._dirty.clear()
 
     def check(self) -> None:
-        """No slot or page lost, held twice, or owned by two sequences."""
+        """No slot or page lost, held twice, or owned by two sequences that did not fork."""
         self.slots.check()
         self.pages.check()
-        seen = set()
+        seen, held = set(), {}
         for slot in range(self.max_sequences):
             owned = self._owned[slot]
             if owned and not self.slots.is_held(slot):
                 raise AssertionError(f"closed slot {slot} still owns pages")
             for page in owned:
-                if page in seen:
+                held[page] = held.get(page, 0) + 1
+                if page in seen and page not in self._holders:
                     raise AssertionError(f"page {page} is owned twice")
                 if not self.pages.is_held(page):
                     raise AssertionError(f"page {page} is owned by slot {slot} but marked free")
                 seen.add(page)
+        for page, holders in self._holders.items():
+            if holders < 2 or held.get(page, 0) != holders:
+                raise AssertionError(f"page {page} is owned {held.get(page, 0)} times, {holders} are counted")
         if len(seen) != self.pages.held_count:
             raise AssertionError("a held page belongs to no sequence")

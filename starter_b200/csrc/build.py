@@ -66,6 +66,9 @@ SOURCES = (
     "state_scan",
     "state_scan_prompt",
     "state_step",
+    "attention_tree",
+    "cache_pages",
+    "token_logprobs",
 )
 
 _lock = threading.Lock()

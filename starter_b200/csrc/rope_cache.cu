@@ -6,7 +6,8 @@
 // the gain), then rotated half-split: out[j] = n[j]*cos[j] - n[j+half]*sin[j], out[j+half] =
 // n[j+half]*cos[j] + n[j]*sin[j], each product and the sum rounded to the working type, cos and sin
 // rounded to the working type first.  Values are copied unchanged.  The cache position of a token is
-// its absolute position in its sequence: page block_table[slot][pos / 64], offset pos % 64.
+// its place in its sequence (its absolute position, but for the nodes of drafted trees): page block_table[slot][place / 64], offset
+// place % 64.
 #include "common.cuh"
 
 #define SB_MAX_PAIRS 4  // head_dim <= 256
@@ -16,13 +17,14 @@ __global__ void qk_norm_rope_store_kernel(
     const T* __restrict__ qkv, T* __restrict__ q_out, const W* __restrict__ q_gain,
     const W* __restrict__ k_gain, const float* __restrict__ cos_table,
     const float* __restrict__ sin_table, const int* __restrict__ tok_pos,
-    const int* __restrict__ tok_slot, const int* __restrict__ block_table, int table_stride,
+    const int* __restrict__ tok_place, const int* __restrict__ tok_slot, const int* __restrict__ block_table, int table_stride,
     T* __restrict__ k_store, T* __restrict__ v_store, int n_tokens, int heads, int kv_heads,
     int head_dim, float eps, int heads_per_token, int row_stride) {
   pdl_trigger();
   pdl_wait();
   SB_BEHIND_WAIT(qkv);
   SB_BEHIND_WAIT(tok_pos);
+  SB_BEHIND_WAIT(tok_place);
   SB_BEHIND_WAIT(tok_slot);
   const int warp = (blockIdx.x * blockDim.x + threadIdx.x) >> 5;
   const int lane = threadIdx.x & 31;
@@ -40,9 +42,10 @@ __global__ void qk_norm_rope_store_kernel(
     dst = q_out + ((size_t)token * heads + h) * head_dim;
   } else {
     const int kvh = is_v ? h - heads - kv_heads : h - heads;
-    const int page = block_table[(size_t)tok_slot[token] * table_stride + pos / SB_PAGE_TOKENS];
+    const int place = tok_place[token];
+    const int page = block_table[(size_t)tok_slot[token] * table_stride + place / SB_PAGE_TOKENS];
     T* store = is_v ? v_store : k_store;
-    dst = store + page_row(page, kvh, pos % SB_PAGE_TOKENS, kv_heads, head_dim);
+    dst = store + page_row(page, kvh, place % SB_PAGE_TOKENS, kv_heads, head_dim);
   }
 
   if (is_v) {
@@ -147,13 +150,14 @@ __global__ void qk_norm_rope_store_vec_kernel(
     const bf16* __restrict__ qkv, bf16* __restrict__ q_out, const W* __restrict__ q_gain,
     const W* __restrict__ k_gain, const float* __restrict__ cos_table,
     const float* __restrict__ sin_table, const int* __restrict__ tok_pos,
-    const int* __restrict__ tok_slot, const int* __restrict__ block_table, int table_stride,
+    const int* __restrict__ tok_place, const int* __restrict__ tok_slot, const int* __restrict__ block_table, int table_stride,
     bf16* __restrict__ k_store, bf16* __restrict__ v_store, long long n_rows, int heads, int kv_heads,
     float eps, int heads_per_token, int row_stride) {
   pdl_trigger();
   pdl_wait();
   SB_BEHIND_WAIT(qkv);
   SB_BEHIND_WAIT(tok_pos);
+  SB_BEHIND_WAIT(tok_place);
   SB_BEHIND_WAIT(tok_slot);
   constexpr int HALF = L * 8, D = 2 * HALF;
   // grid (tokens, blocks of heads): no index needs a division
@@ -171,8 +175,9 @@ __global__ void qk_norm_rope_store_vec_kernel(
     dst = q_out + ((size_t)token * heads + h) * D;
   } else {
     const int kvh = is_v ? h - heads - kv_heads : h - heads;
-    const int page = block_table[(size_t)tok_slot[token] * table_stride + pos / SB_PAGE_TOKENS];
-    dst = (is_v ? v_store : k_store) + page_row(page, kvh, pos % SB_PAGE_TOKENS, kv_heads, D);
+    const int place = tok_place[token];
+    const int page = block_table[(size_t)tok_slot[token] * table_stride + place / SB_PAGE_TOKENS];
+    dst = (is_v ? v_store : k_store) + page_row(page, kvh, place % SB_PAGE_TOKENS, kv_heads, D);
   }
   dst += part * 8;
   uint4 raw_lo = *reinterpret_cast<const uint4*>(src);
@@ -230,7 +235,7 @@ __global__ void qk_norm_rope_store_vec_kernel(
 template <typename W, int L>
 static int launch_vec(const void* qkv, void* q_out, const void* q_gain, const void* k_gain,
                       const float* cos_table, const float* sin_table, const int* tok_pos,
-                      const int* tok_slot, const int* block_table, int table_stride, void* k_store,
+                      const int* tok_place, const int* tok_slot, const int* block_table, int table_stride, void* k_store,
                       void* v_store, int n_tokens, int heads, int kv_heads, float eps, int write_cache,
                       int row_stride, cudaStream_t s) {
   const int per_token = write_cache ? heads + 2 * kv_heads : heads;
@@ -240,17 +245,17 @@ static int launch_vec(const void* qkv, void* q_out, const void* q_gain, const vo
   const int head_blocks = (per_token * L + threads - 1) / threads;
   return launch_dependent(qk_norm_rope_store_vec_kernel<W, L>, dim3((unsigned)n_tokens, (unsigned)head_blocks), dim3(threads), 0, s,
       (const bf16*)qkv, (bf16*)q_out, (const W*)q_gain, (const W*)k_gain, cos_table, sin_table, tok_pos,
-      tok_slot, block_table, table_stride, (bf16*)k_store, (bf16*)v_store, rows, heads, kv_heads, eps,
+      tok_place, tok_slot, block_table, table_stride, (bf16*)k_store, (bf16*)v_store, rows, heads, kv_heads, eps,
       per_token, row_stride);
 }
 
 template <typename W>
 static int launch_vec_by_dim(int head_dim, const void* qkv, void* q_out, const void* q_gain,
                              const void* k_gain, const float* cos_table, const float* sin_table,
-                             const int* tok_pos, const int* tok_slot, const int* block_table,
+                             const int* tok_pos, const int* tok_place, const int* tok_slot, const int* block_table,
                              int table_stride, void* k_store, void* v_store, int n_tokens, int heads,
                              int kv_heads, float eps, int write_cache, int row_stride, cudaStream_t s) {
-#define VARGS qkv, q_out, q_gain, k_gain, cos_table, sin_table, tok_pos, tok_slot, block_table, \
+#define VARGS qkv, q_out, q_gain, k_gain, cos_table, sin_table, tok_pos, tok_place, tok_slot, block_table, \
               table_stride, k_store, v_store, n_tokens, heads, kv_heads, eps, write_cache, row_stride, s
   switch (head_dim) {
     case 16: return launch_vec<W, 1>(VARGS);
@@ -266,7 +271,7 @@ static int launch_vec_by_dim(int head_dim, const void* qkv, void* q_out, const v
 template <typename T, typename W>
 static int launch(const void* qkv, void* q_out, const void* q_gain, const void* k_gain,
                   const float* cos_table, const float* sin_table, const int* tok_pos,
-                  const int* tok_slot, const int* block_table, int table_stride, void* k_store,
+                  const int* tok_place, const int* tok_slot, const int* block_table, int table_stride, void* k_store,
                   void* v_store, int n_tokens, int heads, int kv_heads, int head_dim, float eps,
                   int write_cache, int row_stride, cudaStream_t s) {
   const int per_token = write_cache ? heads + 2 * kv_heads : heads;
@@ -276,7 +281,7 @@ static int launch(const void* qkv, void* q_out, const void* q_gain, const void* 
   const long long blocks = (warps * 32 + threads - 1) / threads;
   return launch_dependent(qk_norm_rope_store_kernel<T, W>, dim3((unsigned)blocks), dim3(threads), 0, s,
       (const T*)qkv, (T*)q_out, (const W*)q_gain, (const W*)k_gain, cos_table, sin_table, tok_pos,
-      tok_slot, block_table, table_stride, (T*)k_store, (T*)v_store, n_tokens, heads, kv_heads,
+      tok_place, tok_slot, block_table, table_stride, (T*)k_store, (T*)v_store, n_tokens, heads, kv_heads,
       head_dim, eps, per_token, row_stride);
 }
 
@@ -285,15 +290,16 @@ extern "C" {
 // qkv: [n_tokens, (heads + 2*kv_heads) * head_dim]; q_out: [n_tokens, heads * head_dim].
 // q_gain / k_gain may be null (no per-head norm); cos_table / sin_table [positions, head_dim/2]
 // float may be null (no rotation).  Rows of qkv are row_stride elements apart.  With
-// write_cache == 0 only the query heads are processed, so qkv may hold the queries alone.
+// write_cache == 0 only the query heads are processed, so qkv may hold the queries alone.  tok_place: the place in its sequence at which a
+// token's key and value are filed (tok_pos itself unless several nodes of a drafted tree stand at one position).
 int sb_qk_norm_rope_store(int dtype, int gain_dtype, const void* qkv, void* q_out, const void* q_gain,
                           const void* k_gain, const float* cos_table, const float* sin_table,
-                          const int* tok_pos, const int* tok_slot, const int* block_table,
+                          const int* tok_pos, const int* tok_place, const int* tok_slot, const int* block_table,
                           int table_stride, void* k_store, void* v_store, int n_tokens, int heads,
                           int kv_heads, int head_dim, float eps, int write_cache, int row_stride,
                           cudaStream_t s) {
   if (head_dim > 64 * SB_MAX_PAIRS || (head_dim & 1)) return -2;
-#define ARGS qkv, q_out, q_gain, k_gain, cos_table, sin_table, tok_pos, tok_slot, block_table, \
+#define ARGS qkv, q_out, q_gain, k_gain, cos_table, sin_table, tok_pos, tok_place, tok_slot, block_table, \
              table_stride, k_store, v_store, n_tokens, heads, kv_heads, head_dim, eps, write_cache, \
              row_stride, s
   // bfloat16 with a power-of-two head size and 16-byte aligned rows takes the 16-byte kernel
@@ -304,11 +310,11 @@ int sb_qk_norm_rope_store(int dtype, int gain_dtype, const void* qkv, void* q_ou
   if (dtype == 1 && pow2 && aligned) {
     if (gain_dtype == 1)
       return launch_vec_by_dim<bf16>(head_dim, qkv, q_out, q_gain, k_gain, cos_table, sin_table, tok_pos,
-                                     tok_slot, block_table, table_stride, k_store, v_store, n_tokens,
+                                     tok_place, tok_slot, block_table, table_stride, k_store, v_store, n_tokens,
                                      heads, kv_heads, eps, write_cache, row_stride, s);
     if (gain_dtype == 0)
       return launch_vec_by_dim<float>(head_dim, qkv, q_out, q_gain, k_gain, cos_table, sin_table, tok_pos,
-                                      tok_slot, block_table, table_stride, k_store, v_store, n_tokens,
+                                      tok_place, tok_slot, block_table, table_stride, k_store, v_store, n_tokens,
                                       heads, kv_heads, eps, write_cache, row_stride, s);
   }
   if (dtype == 0 && gain_dtype == 0) return launch<float, float>(ARGS);

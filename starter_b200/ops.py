@@ -504,13 +504,15 @@ def rotation_tables(rotation, head_dim: int):
 
 
 def qk_norm_rope_store(qkv, heads, kv_heads, head_dim, q_gain, k_gain, eps, cos_table, sin_table,
-                       tok_pos, tok_slot, block_table, k_store, v_store, write_cache=True):
+                       tok_pos, tok_slot, block_table, k_store, v_store, write_cache=True, tok_place=None):
     """Norm and rotate the query and key heads of ``qkv`` and file keys and values in the cache.
 
     ``qkv`` is ``[T, (heads + 2 * kv_heads) * head_dim]`` (queries alone,
     ``[T, heads * head_dim]``, when ``write_cache`` is false); returns the queries
     ``[T, heads * head_dim]``.  ``k_store``/``v_store`` are one cache entry's pages
-    ``[pages, kv_heads, 64, head_dim]``; ``block_table`` int32 ``[slots, max_pages]``.
+    ``[pages, kv_heads, 64, head_dim]``; ``block_table`` int32 ``[slots, max_pages]``.  ``tok_pos`` are the
+    positions the heads are rotated to, ``tok_place`` (None: the same) the places of their sequence
+    that keys and values are filed at; they differ for the nodes of a drafted tree.
     """
     _need(qkv, "qkv", None, 2)
     n_tokens = qkv.shape[0]
@@ -521,6 +523,12 @@ def qk_norm_rope_store(qkv, heads, kv_heads, head_dim, q_gain, k_gain, eps, cos_
         raise KernelError(f"head_dim {head_dim} must be even and at most {MAX_HEAD_DIM}")
     _need(tok_pos, "tok_pos", torch.int32, 1)
     _need(tok_slot, "tok_slot", torch.int32, 1)
+    if tok_place is None:
+        tok_place = tok_pos
+    else:
+        _need(tok_place, "tok_place", torch.int32, 1)
+        if tok_place.shape != tok_pos.shape:
+            raise KernelError(f"{tok_place.shape[0]} places for {tok_pos.shape[0]} positions")
     _need(block_table, "block_table", torch.int32, 2)
     gain_code = 0
     for g in (q_gain, k_gain):
@@ -545,7 +553,7 @@ def qk_norm_rope_store(qkv, heads, kv_heads, head_dim, q_gain, k_gain, eps, cos_
     q_out = _empty(qkv, (n_tokens, heads * head_dim))
     rc = _lib("rope_cache").sb_qk_norm_rope_store(
         _code(qkv.dtype), gain_code, qkv, q_out, q_gain, k_gain,
-        cos_table, sin_table, tok_pos, tok_slot, block_table,
+        cos_table, sin_table, tok_pos, tok_place, tok_slot, block_table,
         block_table.shape[1], k_store if write_cache else None,
         v_store if write_cache else None, n_tokens, heads, kv_heads, head_dim,
         eps, int(write_cache), qkv.shape[1], _stream())
@@ -1207,6 +1215,254 @@ def sample(logits, temperature=None, request_key=None, position=None, status=Non
         feed[2] if feed else None, cand_v, cand_i, _stream())
     _check(rc, "sample", 2)
     return out
+
+
+# ---------------------------------------------------------------------------------------- log probabilities
+
+def _here(t, name):
+    """Refuse an operand of another device than the current one, on whose stream the kernel would run."""
+    if t.get_device() != torch.cuda.current_device():
+        raise KernelError(f"{name} is on {t.device}; the current device is cuda:{torch.cuda.current_device()}")
+
+
+#: the most alternatives ``token_logprobs`` lists
+LOGPROBS_MAX_TOP = 32
+
+
+def _logprob_parts(rows: int, vocab: int) -> int:
+    """How many blocks (a cluster) share a row of logits: as many as keep two blocks on every SM."""
+    parts = 1
+    while parts < 8 and 2 * parts * rows <= 2 * SM_COUNT and 2 * parts * 4096 <= vocab:
+        parts *= 2
+    return parts
+
+
+def token_logprobs(logits, tokens, top=0, status=None):
+    """What a model's logits say of given tokens: ``(logprob, entropy, top_logprobs, top_ids)``.
+
+    ``logits`` ``[R, V]``, float32 or bfloat16, whose rows may lie further apart than V entries; ``tokens`` int32 ``[R]``.  With
+    ``p = softmax(logits[r])``: ``logprob[r] = log p[tokens[r]]`` and ``entropy[r] = -sum p log p`` (float32 ``[R]``), and the ``top``
+    largest entries (at most ``LOGPROBS_MAX_TOP``, largest first, the lowest index first among equals) as ``top_logprobs`` float32
+    and ``top_ids`` int32 ``[R, top]``.  A negative token stands for none and has the log probability 0; one of V or more has none
+    (not a number) and sets bit 1 of ``status``.  Entries of minus infinity have the probability 0; entries that are no numbers make a
+    row's results no numbers and are not listed (places left over hold the index -1)."""
+    _refuse_rows(logits, "logits")
+    _need(tokens, "tokens", torch.int32, 1)
+    _here(logits, "logits")
+    rows, vocab = logits.shape
+    top = int(top)
+    if tokens.shape[0] != rows:
+        raise KernelError(f"{tokens.shape[0]} tokens for {rows} rows of logits")
+    if not 0 <= top <= min(LOGPROBS_MAX_TOP, vocab):
+        raise KernelError(f"{top} alternatives asked for; the kernel lists 0 to {min(LOGPROBS_MAX_TOP, vocab)} of {vocab}")
+    out = _empty(tokens, (2, rows), torch.float32)
+    values, ids = _empty(tokens, (rows, top), torch.float32), _empty(tokens, (rows, top), torch.int32)
+    if rows:
+        rc = _lib("token_logprobs").sb_token_logprobs(
+            _code(logits.dtype), logits, rows, vocab, logits.stride(0), tokens, top, out[0], out[1], values, ids,
+            _logprob_parts(rows, vocab), status, _stream())
+        _check(rc, "token_logprobs", -(-rows // 65535))
+    return out[0], out[1], values, ids
+
+
+def _refuse_rows(t, name):
+    """Refuse what is no CUDA matrix with contiguous rows (which may lie further apart than they are long)."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise KernelError(f"{name} must be a CUDA tensor (there is no CPU implementation)")
+    if t.dim() != 2 or t.shape[1] == 0:
+        raise KernelError(f"{name} must have 2 dimensions and rows that are not empty, got shape {tuple(t.shape)}")
+    _code(t.dtype)
+    if (t.stride(1) != 1 and t.shape[1] > 1) or (t.stride(0) < t.shape[1] and t.shape[0] > 1):
+        raise KernelError(f"the rows of {name} must be contiguous, got strides {t.stride()} for shape {tuple(t.shape)}")
+
+
+#: bytes of logits that ``linear_logprobs`` forms at a time where it forms any
+LOGPROBS_CHUNK_BYTES = 256 << 20
+
+
+def linear_logprobs(h, weight, tokens, softcap=None, status=None):
+    """``token_logprobs`` of ``h @ weight.T`` without alternatives: ``(logprob, entropy)``, float32 ``[R]`` each.
+
+    ``h`` ``[R, K]`` are hidden rows behind the final norm, ``weight`` ``[V, K]`` the head, of the same type; ``softcap`` (None: none)
+    caps the logits as ``ops.softcap`` does."""
+    _need(h, "h", None, 2)
+    _need(weight, "weight", h.dtype, 2)
+    _need(tokens, "tokens", torch.int32, 1)
+    _here(h, "h")
+    rows, vocab = h.shape[0], weight.shape[0]
+    if weight.shape[1] != h.shape[1]:
+        raise KernelError(f"weight {tuple(weight.shape)} does not take inputs of width {h.shape[1]}")
+    if tokens.shape[0] != rows:
+        raise KernelError(f"{tokens.shape[0]} tokens for {rows} rows")
+    if vocab == 0 or h.shape[1] == 0:
+        raise KernelError(f"a head of shape {tuple(weight.shape)} gives no logits")
+    out = _empty(h, (2, rows), torch.float32)
+    chunk = max(1, LOGPROBS_CHUNK_BYTES // (4 * vocab))
+    for first in range(0, rows, chunk):
+        logits = linear(h[first:first + chunk], weight, out_float=True, status=status)
+        if softcap is not None:
+            globals()["softcap"](logits, softcap)
+        out[0, first:first + chunk], out[1, first:first + chunk] = token_logprobs(logits, tokens[first:first + chunk], status=status)[:2]
+    return out[0], out[1]
+
+
+# ---------------------------------------------------------------------------------------- drafted trees
+
+#: the most nodes a sequence's tree may have
+TREE_MAX_NODES = 256
+
+
+def _tree_step(block_table, seq_slot, seq_q_start, seq_q_len, seq_kv_len, max_q_len):
+    """Check a step's sequence arrays; returns how many sequences there are."""
+    _need(block_table, "block_table", torch.int32, 2)
+    for name, t in (("seq_slot", seq_slot), ("seq_q_start", seq_q_start), ("seq_q_len", seq_q_len), ("seq_kv_len", seq_kv_len)):
+        _need(t, name, torch.int32, 1)
+        if t.shape[0] != seq_slot.shape[0]:
+            raise KernelError(f"{name} has {t.shape[0]} entries for {seq_slot.shape[0]} sequences")
+    if not 1 <= max_q_len <= TREE_MAX_NODES:
+        raise KernelError(f"trees of {max_q_len} nodes; the kernels take 1 to {TREE_MAX_NODES}")
+    return seq_slot.shape[0]
+
+
+@functools.lru_cache(maxsize=4096)
+def _tree_plain_splits(blocks: int, keys: int) -> int:
+    return max(1, min(-(-keys // 64), 592 // max(blocks, 1), 32))
+
+
+def attention_tree(q, k_store, v_store, block_table, seq_slot, seq_q_start, seq_q_len, seq_kv_len, tok_pos, tree_mask, heads, kv_heads,
+                   head_dim, scale, window=None, max_q_len=None, kv_hint=0, status=None):
+    """Attention of the nodes of drafted trees over the paged cache.
+
+    ``q`` ``[T, heads * head_dim]`` packed by sequence; the ``seq_*`` arrays describe each sequence of the step as they do for
+    ``attention_prefill``: its nodes are the rows ``seq_q_start`` to ``+ seq_q_len``, their keys and values are filed behind its
+    ``seq_kv_len - seq_q_len`` cached tokens, node i's at place ``seq_kv_len - seq_q_len + i``.  ``tok_pos`` int32 ``[T]`` are the nodes'
+    positions (cached tokens plus depth).  Every node sees the cached tokens and, of its sequence's nodes, those whose bit is set in its
+    row of ``tree_mask`` (int32 ``[T, words]``, node m is bit m % 32 of word m // 32); with ``window`` only what lies less than
+    ``window`` positions before it.  A node that sees nothing gets zeros.  ``max_q_len``: the longest ``seq_q_len`` (at most
+    ``TREE_MAX_NODES``; by default what the words hold); rows that belong to no sequence hold nothing.  ``kv_hint``: the longest
+    ``seq_kv_len``, by which the keys are cut into parts (wrong, it costs time only)."""
+    _need(q, "q", None, 2)
+    _here(q, "q")
+    code = _code(q.dtype)
+    if kv_heads < 1 or heads % kv_heads:
+        raise KernelError(f"{heads} query heads cannot share {kv_heads} key/value heads")
+    if q.shape[1] != heads * head_dim:
+        raise KernelError(f"q has width {q.shape[1]}, expected {heads * head_dim}")
+    if not 1 <= head_dim <= MAX_HEAD_DIM:
+        raise KernelError(f"head_dim {head_dim} exceeds {MAX_HEAD_DIM}")
+    for store in (k_store, v_store):
+        _need(store, "cache pages", q.dtype, 4)
+        if tuple(store.shape[1:]) != (kv_heads, PAGE_TOKENS, head_dim):
+            raise KernelError(f"cache pages have shape {tuple(store.shape)}")
+    _need(tok_pos, "tok_pos", torch.int32, 1)
+    _need(tree_mask, "tree_mask", torch.int32, 2)
+    words = tree_mask.shape[1]
+    if tok_pos.shape[0] != q.shape[0] or tree_mask.shape[0] != q.shape[0]:
+        raise KernelError(f"{q.shape[0]} rows with {tok_pos.shape[0]} positions and {tree_mask.shape[0]} masks")
+    if max_q_len is None:
+        max_q_len = min(32 * words, TREE_MAX_NODES)
+    seqs = _tree_step(block_table, seq_slot, seq_q_start, seq_q_len, seq_kv_len, max_q_len)
+    if 32 * words < max_q_len:
+        raise KernelError(f"masks of {words} words for trees of {max_q_len} nodes")
+    if window is not None and window < 1:
+        raise KernelError(f"a window of {window}")
+    out = _empty(q, q.shape)
+    if q.shape[0] == 0 or seqs == 0:
+        return out
+    group = heads // kv_heads
+    splits = _tree_plain_splits(-(-max_q_len * group // 16) * kv_heads * seqs, min(kv_hint, window + max_q_len) if window else kv_hint)
+    acc = ml = None
+    if splits > 1:
+        acc = _empty(q, (q.shape[0] * heads * splits * head_dim,), torch.float32)
+        ml = _empty(q, (q.shape[0] * heads * splits * 2,), torch.float32)
+    rc = _lib("attention_tree").sb_attention_tree_plain(
+        code, q, out, k_store, v_store, block_table, block_table.shape[1], seq_slot, seq_q_start, seq_q_len, seq_kv_len, tok_pos, tree_mask,
+        words, seqs, max_q_len, heads, kv_heads, head_dim, scale, int(window or 0), splits, acc, ml, _stream())
+    _check(rc, "attention_tree", 2 if splits > 1 else 1)
+    return out
+
+
+def cache_accept(stores, block_table, seq_slot, seq_q_start, seq_q_len, seq_kv_len, tokens, parents, drawn, max_q_len):
+    """Walk every sequence's drafted tree down by what was drawn, and move the cache rows of the nodes on the way together.
+
+    The step is described as for ``attention_tree``.  ``tokens``, ``parents`` and ``drawn`` (int32 ``[T]``): each node's token, the node of
+    its sequence it hangs on (below its own number; the first node is the root and hangs on none, -1), and the token that was drawn behind it.
+    From the root the walk goes on to the child whose token was drawn at its parent (the lowest such child) until there is none.  The i-th
+    node on the way has its keys and values at place ``past + node`` of its sequence; they are moved to ``past + i`` in every tensor pair
+    of ``stores`` (``(keys, values)``, ``[entries, pages, kv_heads, 64, dim]``, a cache group's storage, or one entry's without the first
+    dimension).  Returns int32 ``count`` ``[S]`` (nodes on the way), ``path`` ``[S, max_q_len]`` (which ones, then -1) and ``taken``
+    ``[S, max_q_len]`` (what was drawn at each, then -1): the sequence has ``past + count`` tokens now and goes on with
+    ``taken[count - 1]``.  ``max_q_len``: the longest ``seq_q_len``, at most ``TREE_MAX_NODES``."""
+    seqs = _tree_step(block_table, seq_slot, seq_q_start, seq_q_len, seq_kv_len, max_q_len)
+    for name, t in (("tokens", tokens), ("parents", parents), ("drawn", drawn)):
+        _need(t, name, torch.int32, 1)
+        if t.shape[0] != tokens.shape[0]:
+            raise KernelError(f"{name} has {t.shape[0]} entries for {tokens.shape[0]} nodes")
+    _here(tokens, "tokens")
+    geometry = []
+    for keys, values in stores:
+        for t in (keys, values):
+            _need(t, "cache pages")
+            if t.dim() not in (4, 5) or t.shape[-2] != PAGE_TOKENS or t.shape[:-1] != keys.shape[:-1] or t.numel() == 0:
+                raise KernelError(f"cache pages have shapes {tuple(keys.shape)} and {tuple(values.shape)}")
+        rows = [t.shape[-1] * t.element_size() for t in (keys, values)]
+        if rows[0] % 4 or rows[1] % 4 or keys.data_ptr() % 4 or values.data_ptr() % 4:
+            raise KernelError(f"rows of {rows[0]} and {rows[1]} bytes: the kernel moves words of four")
+        geometry.append((keys, values, rows, keys.shape[0] if keys.dim() == 5 else 1, keys.shape[-4], keys.shape[-3]))
+    if not geometry:
+        raise KernelError("no cache pages are given")
+    count = _empty(tokens, (seqs,))
+    ways = _empty(tokens, (2, seqs, max_q_len))
+    outs = (count, ways[0], ways[1])
+    if seqs:
+        lib = _lib("cache_pages")
+        for n, (keys, values, rows, entries, pages, kv_heads) in enumerate(geometry):
+            count_to, path_to, taken_to = outs if n == 0 else (None, None, None)
+            rc = lib.sb_cache_accept(keys, values, rows[0], rows[1], entries, pages, kv_heads, block_table, block_table.shape[1], seq_slot,
+                                     seq_q_start, seq_q_len, seq_kv_len, seqs, tokens, parents, drawn, count_to, path_to, taken_to,
+                                     max_q_len, _stream())
+            _check(rc, "cache_accept")
+    return outs
+
+
+# ---------------------------------------------------------------------------------------- pages
+
+def cache_copy_pages(stores, source, target, dim=1):
+    """Copy page ``source[i]`` to page ``target[i]`` (host integers) in every tensor of ``stores``, for all i at once.
+
+    ``stores`` are contiguous tensors of a cache group's storage ``[entries, pages, ...]``; ``dim`` says which dimension counts the pages (0:
+    one entry's ``[pages, ...]``, or a state ``[slots, ...]``).  No target may be named twice or be a source: the copies are made in any order."""
+    source, target = [int(p) for p in source], [int(p) for p in target]
+    if len(source) != len(target):
+        raise KernelError(f"{len(source)} pages to copy to {len(target)}")
+    if len(set(target)) < len(target) or set(target) & set(source):
+        raise KernelError("a page is copied to twice, or from and to")
+    if dim not in (0, 1):
+        raise KernelError(f"pages are counted by the first or the second dimension, not {dim}")
+    described = []
+    for t in stores:
+        _need(t, "cache pages")
+        _here(t, "cache pages")
+        if t.dim() <= dim:
+            raise KernelError(f"cache pages have shape {tuple(t.shape)}")
+        items = t.shape[dim]
+        if source and not (0 <= min(min(source), min(target)) and max(max(source), max(target)) < items):
+            raise KernelError(f"a page outside the {items} of the cache")
+        if t.numel() == 0:                       # (a latent's cache keeps no values)
+            continue
+        outer = t.shape[0] if dim else 1
+        described += [t.data_ptr(), outer, items, t.numel() // (outer * items) * t.element_size()]
+    if not source or not described:
+        return
+    lib = _lib("cache_pages")
+    per_tensors, per_pairs = 16, 256
+    pairs = [n for pair in zip(source, target) for n in pair]
+    for t in range(0, len(described), 4 * per_tensors):
+        some = (ctypes.c_longlong * len(described[t:t + 4 * per_tensors]))(*described[t:t + 4 * per_tensors])
+        for p in range(0, len(pairs), 2 * per_pairs):
+            here = (ctypes.c_int * len(pairs[p:p + 2 * per_pairs]))(*pairs[p:p + 2 * per_pairs])
+            rc = lib.sb_cache_copy(ctypes.addressof(some), len(some) // 4, ctypes.addressof(here), len(here) // 2, _stream())
+            _check(rc, "cache_copy_pages")
 
 
 # ---------------------------------------------------------------------------------------- chains
