@@ -7,7 +7,7 @@ __version__ = "0.1.0"
 
 def __getattr__(name):
     # the entry point needs torch and the kernels; import it on first use
-    if name in ("Engine", "Completion", "Request", "SamplingParams"):
+    if name in ("Engine", "Completion", "Request", "SamplingParams", "ScoredTokens"):
         from .engine import entry
         return getattr(entry, name)
     raise AttributeError(f"module 'starter_b200' has no attribute {name!r}")

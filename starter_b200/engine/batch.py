@@ -16,6 +16,8 @@ import numpy as np
 import torch
 
 
+#: the most nodes of a drafted tree (the attention's and the cache's kernels take no more)
+TREE_MAX_NODES = 256
 QUERY_TILE = 64
 QUERY_BLOCK = 256      # what one block of the tensor-core prompt attention takes
 
@@ -32,6 +34,21 @@ class StepEntry:
     slot: int
     tokens: list
     want: list = field(default_factory=list)
+
+
+@dataclass
+class TreeEntry:
+    """One sequence's share of a step with drafts: its slot, the tokens of a tree's nodes and each node's parent
+    (its place among the nodes, below the node's own).  Node 0 is the root, the sequence's next token, and has the
+    parent -1; every other node is a draft of what may follow its parent."""
+
+    slot: int
+    tokens: list
+    parents: list
+
+    @property
+    def want(self):
+        return range(len(self.tokens))
 
 
 @dataclass
@@ -63,6 +80,11 @@ class StepContext:
     #: earlier steps wrote is then complete before any kernel of this step starts, and a kernel may
     #: read it before its own dependent-launch wait.  Set by the model; False for a context made by hand.
     fenced: bool = False
+    #: in a step with drafted trees (``plan_trees``): which nodes every node sees, as bits, and the place of
+    #: its sequence that its key and value are filed at (its position, ``tok_pos``, goes by its depth)
+    tree_mask: torch.Tensor = None
+    tok_place: torch.Tensor = None
+    parents: torch.Tensor = None
 
     @property
     def is_decode(self) -> bool:
@@ -114,6 +136,41 @@ def plan_step(entries, starts, vocab_size=None):
         "block_seq": [t[1] for t in blocks], "block_first": [t[2] for t in blocks],
     }
     return {k: np.asarray(v, dtype=np.int32) for k, v in arrays.items()}
+
+
+def plan_trees(entries, starts, vocab_size=None):
+    """``plan_step`` for a step with drafted trees (``TreeEntry``): every node is a row whose logits are wanted.
+
+    Besides the arrays of ``plan_step``, with positions that go by depth: ``tok_place`` (where a node's key and value
+    are filed: behind the cached tokens, node by node), ``parents`` and ``tree_mask`` (bit m of a node's words: itself
+    or a node above it, flattened ``[rows, words]``)."""
+    for entry in entries:
+        n = len(entry.tokens)
+        if len(entry.parents) != n:
+            raise ValueError(f"the tree in slot {entry.slot} has {n} tokens and {len(entry.parents)} parents")
+        if n > TREE_MAX_NODES:
+            raise ValueError(f"the tree in slot {entry.slot} has {n} nodes; {TREE_MAX_NODES} are the most")
+        if n and entry.parents[0] != -1:
+            raise ValueError(f"the first node of the tree in slot {entry.slot} is its root: its parent is -1, not {entry.parents[0]}")
+        for i, parent in enumerate(entry.parents):
+            if i and not 0 <= parent < i:
+                raise ValueError(f"node {i} of the tree in slot {entry.slot} hangs on {parent}: a parent stands before its node")
+    arrays = plan_step(entries, starts, vocab_size)
+    words = -(-max(len(e.tokens) for e in entries) // 32)
+    position, masks, parents = [], [], []
+    for entry, start in zip(entries, starts):
+        depth, bits = [], []
+        for i, parent in enumerate(entry.parents):
+            depth.append(depth[parent] + 1 if i else 0)
+            bits.append((bits[parent] if i else 0) | 1 << i)
+        position.extend(start + d for d in depth)
+        masks.extend(b.to_bytes(4 * words, "little") for b in bits)
+        parents.extend(entry.parents)
+    arrays["tok_place"] = arrays["tok_pos"]
+    arrays["tok_pos"] = np.asarray(position, dtype=np.int32)
+    arrays["parents"] = np.asarray(parents, dtype=np.int32)
+    arrays["tree_mask"] = np.frombuffer(b"".join(masks), dtype="<i4").astype(np.int32)
+    return arrays
 
 
 def upload(arrays: dict, device) -> dict:

@@ -17,8 +17,8 @@ import torch
 
 from ..cache.layout import PAGE_TOKENS
 from ..sampling.sampler import Sampler, SamplingParams
-from .generate import Completion, GenerationLoop, Request, pages_held
-from .runner import ModelRunner, load_model
+from .generate import Completion, GenerationLoop, Request, pages_held, plan_batches
+from .runner import ModelRunner, ScoredTokens, load_model
 
 
 class Engine:
@@ -103,5 +103,19 @@ class Engine:
         self.runner.check_status()
         return out
 
+    @torch.inference_mode()
+    def score(self, input_ids: list, top: int = 0) -> list:
+        """What the model says of given texts: a ``ScoredTokens`` per text (log probabilities of its tokens, entropies, and the
+        ``top`` likeliest tokens at every place).  Texts run in batches of at most ``max_batch``, one batch after another."""
+        requests = [Request(list(ids), 1) for ids in input_ids]
+        if not requests:
+            return []
+        loop = self._ensure_room(requests, min(self.max_batch, len(requests)))
+        out = []
+        for batch in plan_batches(requests, loop.max_batch, loop.max_pages):
+            out.extend(self.runner.score([requests[i].prompt for i in batch], top))
+        self.runner.check_status()
+        return out
 
-__all__ = ["Completion", "Engine", "Request", "SamplingParams"]
+
+__all__ = ["Completion", "Engine", "Request", "SamplingParams", "ScoredTokens"]

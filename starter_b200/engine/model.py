@@ -231,20 +231,31 @@ class DecoderModel:
                                                          entry.writes_cache)
         return residual, pending
 
-    def logits(self, residual, pending, rows, status=None):
-        """Float32 logits ``[len(rows), vocab]`` of the rows asked for."""
+    def close(self, residual, pending, rows):
+        """The rows asked for behind the final norm, ``[len(rows), width]``: what the head takes."""
         if self.many_streams:
-            h = close_rows(residual, pending, rows, self.final_norm, self.dtype)
-        elif self.float_residual:
-            h = close_rows32(residual, pending, rows, self.final_norm, self.dtype)
-        elif self.depth_residual:
-            h = close_rows_depth(residual, pending, rows, self.final_norm, self.dtype)
-        else:
-            h = self.final_norm.add_rows(residual, pending, rows)
+            return close_rows(residual, pending, rows, self.final_norm, self.dtype)
+        if self.float_residual:
+            return close_rows32(residual, pending, rows, self.final_norm, self.dtype)
+        if self.depth_residual:
+            return close_rows_depth(residual, pending, rows, self.final_norm, self.dtype)
+        return self.final_norm.add_rows(residual, pending, rows)
+
+    def head(self, h, status=None):
+        """Float32 logits ``[rows, vocab]`` of closed rows."""
         logits = ops.linear(h, self.lm_head, out_float=True, status=status)
         if self.spec.logit_softcap is not None:
             ops.softcap(logits, self.spec.logit_softcap)
         return logits
+
+    def logits(self, residual, pending, rows, status=None):
+        """Float32 logits ``[len(rows), vocab]`` of the rows asked for."""
+        return self.head(self.close(residual, pending, rows), status)
+
+    @property
+    def takes_trees(self) -> bool:
+        """Whether every layer's mixer can see the nodes of a drafted tree."""
+        return all(getattr(self.blocks[entry.layer].mixer, "takes_trees", False) for entry in self.spec.schedule)
 
     def forward(self, ctx, rows):
         residual, pending = self.hidden(ctx)

@@ -12,14 +12,18 @@ tokens.  (The reference has two functions for this, ``_forward_prefill`` and
 
 from __future__ import annotations
 
+import contextlib
 import os
+from dataclasses import dataclass
 
+import numpy as np
 import torch
 
+from .. import ops
 from ..cache import SequenceCache, pages_for
 from ..config import load_config
 from ..weights import load_checkpoint
-from .batch import FED, StepContext, StepEntry, plan_step, upload
+from .batch import FED, StepContext, StepEntry, TreeEntry, plan_step, plan_trees, upload
 from .graphs import DecodeGraphs, DrawnTokens
 from .model import DecoderModel
 
@@ -88,6 +92,17 @@ def random_model(config, seed: int, dtype="bfloat16", device="cuda:0") -> Decode
     return model
 
 
+@dataclass
+class ScoredTokens:
+    """What a model says of a text: for every token but the first its log probability behind the tokens before it, the entropy
+    of the model's distribution there, and the likeliest tokens with their log probabilities (empty lists if none were asked for)."""
+
+    logprobs: list
+    entropies: list
+    top_ids: list
+    top_logprobs: list
+
+
 class ModelRunner:
     def __init__(self, model: DecoderModel, max_tokens: int, max_sequences: int | None = None,
                  max_sequence_tokens: int | None = None, use_graphs: bool = True):
@@ -116,6 +131,14 @@ class ModelRunner:
         self.cache.close_sequence(slot)
         self._forget_fed(slot)
 
+    def fork(self, slot: int, count: int = 1, length: int | None = None) -> list:
+        """``count`` sequences that go on from what ``slot`` holds (or its first ``length`` tokens); returns their slots.  Full
+        cache pages are shared, the last one and the state are copied (``SequenceCache.fork``)."""
+        slots = self.cache.fork(slot, count, length)
+        for new in slots:
+            self._forget_fed(new)
+        return slots
+
     def _forget_fed(self, slot: int) -> None:
         """What the device holds as the next input of ``slot`` belongs to a sequence that is gone."""
         graphs = self.graphs
@@ -133,10 +156,10 @@ class ModelRunner:
 
     # ------------------------------------------------------------------ the step
 
-    def make_context(self, entries) -> StepContext:
+    def make_context(self, entries, trees: bool = False) -> StepContext:
         cache = self.cache
         starts = [cache.lengths[e.slot] for e in entries]
-        arrays = plan_step(entries, starts, self.model.spec.vocab_size)
+        arrays = (plan_trees if trees else plan_step)(entries, starts, self.model.spec.vocab_size)
         for e in entries:
             cache.reserve(e.slot, cache.lengths[e.slot] + len(e.tokens))
         for e in entries:
@@ -153,26 +176,110 @@ class ModelRunner:
             tile_seq=dev["tile_seq"], tile_first=dev["tile_first"],
             block_seq=dev["block_seq"], block_first=dev["block_first"],
             max_q_len=int(arrays["seq_q_len"].max()), max_kv_len=max_kv,
-            cache=cache, status=self.status, host=arrays)
+            cache=cache, status=self.status, host=arrays,
+            tree_mask=dev["tree_mask"].view(arrays["tokens"].size, -1) if trees else None,
+            tok_place=dev["tok_place"] if trees else None, parents=dev["parents"] if trees else None)
 
     @torch.inference_mode()
     def step(self, entries) -> torch.Tensor:
         """Run one step; ``entries`` is a list of ``StepEntry``.  Returns ``[wanted, vocab]`` float32."""
         entries = [e if isinstance(e, StepEntry) else StepEntry(*e) for e in entries]
+        with self._step_of(entries):
+            ctx = self.make_context(entries)
+            return self.model.forward(ctx, ctx.want_rows)
+
+    @contextlib.contextmanager
+    def _step_of(self, entries):
+        """A step that raises leaves every sequence as long as it was: tokens whose keys were never (or only partly)
+        written are not counted, and later steps do not read them."""
         if self.graphs is not None:
             self.graphs.fed = None
         cache = self.cache
         before = [(e.slot, cache.lengths[e.slot]) for e in entries]
         try:
-            ctx = self.make_context(entries)
-            return self.model.forward(ctx, ctx.want_rows)
+            yield
         except BaseException:
-            # a step that raises leaves every sequence as long as it was: tokens whose keys were
-            # never (or only partly) written are not counted, and later steps do not read them
             for slot, length in before:
                 if cache.slots.is_held(slot):
                     cache.lengths[slot] = length
             raise
+
+    @torch.inference_mode()
+    def step_trees(self, entries, sampler, temperatures, keys) -> list:
+        """One step with drafted tokens: every ``TreeEntry`` brings its sequence's next token and a tree of drafts behind it.
+
+        All nodes run as one batch, a token is drawn behind each (by the same rule as everywhere: a function of the request's key and the
+        position), and the walk from the root along drafts that were drawn keeps those.  Returns, per entry, the tokens drawn on the way,
+        one or more: the tokens that one-token steps would have drawn, up to the rounding of logits.  The last of them is the
+        sequence's next token; the others and the root are in the cache.  ``temperatures`` and ``keys`` are given per entry."""
+        entries = [e if isinstance(e, TreeEntry) else TreeEntry(*e) for e in entries]
+        if not self.model.takes_trees:
+            raise ValueError("this model has layers that cannot see the nodes of a drafted tree (recurrences, or attention of another kind)")
+        if len(temperatures) != len(entries) or len(keys) != len(entries):
+            raise ValueError(f"{len(entries)} trees with {len(temperatures)} temperatures and {len(keys)} keys")
+        cache = self.cache
+        with self._step_of(entries):
+            ctx = self.make_context(entries, trees=True)
+            logits = self.model.forward(ctx, ctx.want_rows)
+            counts = ctx.host["seq_q_len"]
+            drawn = sampler.select_device(logits, np.repeat(np.asarray(temperatures, dtype=np.float32), counts),
+                                          np.repeat(np.asarray(keys, dtype=np.uint32), counts), ctx.host["tok_pos"] + 1)
+            count, _, taken = ops.cache_accept(list(zip(cache.keys, cache.values)), cache.block_table, ctx.seq_slot, ctx.seq_q_start,
+                                               ctx.seq_q_len, ctx.seq_kv_len, ctx.tokens, ctx.parents, drawn, max_q_len=ctx.max_q_len)
+            both = torch.cat([count[:, None], taken], dim=1).tolist()      # one copy from the device
+        out = []
+        for entry, (n, *tokens) in zip(entries, both):
+            cache.shorten(entry.slot, cache.lengths[entry.slot] - len(entry.tokens) + n)
+            out.append(tokens[:n])
+        return out
+
+    @torch.inference_mode()
+    def score(self, texts, top: int = 0) -> list:
+        """What the model says of every token of the texts (lists of token ids, all run in one step): ``ScoredTokens`` each.
+        The sequences are opened for it and closed again."""
+        texts = [list(t) for t in texts]
+        if not 0 <= top <= min(ops.LOGPROBS_MAX_TOP, self.model.spec.vocab_size):
+            raise ValueError(f"{top} alternatives asked for; 0 to {min(ops.LOGPROBS_MAX_TOP, self.model.spec.vocab_size)} can be listed")
+        if any(len(t) == 0 for t in texts):
+            raise ValueError("a text needs at least one token")
+        if not texts:
+            return []
+        slots = []
+        try:
+            for _ in texts:
+                slots.append(self.open_sequence())
+            entries = [StepEntry(slot, t, list(range(len(t) - 1))) for slot, t in zip(slots, texts)]
+            with self._step_of(entries):
+                ctx = self.make_context(entries)
+                residual, pending = self.model.hidden(ctx)
+                found = self._score_rows(residual, pending, ctx, [t for text in texts for t in text[1:]], top)
+        finally:
+            for slot in slots:
+                self.close_sequence(slot)
+        out, at = [], 0
+        for text in texts:
+            end = at + len(text) - 1
+            out.append(ScoredTokens(*(part[at:end] for part in found)))
+            at = end
+        return out
+
+    def _score_rows(self, residual, pending, ctx, targets, top):
+        """Log probabilities, entropies and alternatives of the wanted rows, as lists."""
+        if not targets:
+            return [], [], [], []
+        model = self.model
+        h = model.close(residual, pending, ctx.want_rows)
+        tokens = torch.tensor(targets, dtype=torch.int32).to(self.device)
+        if top == 0:
+            given, entropy = ops.linear_logprobs(h, model.lm_head, tokens, softcap=model.spec.logit_softcap, status=ctx.status)
+            return given.tolist(), entropy.tolist(), [[] for _ in targets], [[] for _ in targets]
+        parts = []
+        rows = max(1, ops.LOGPROBS_CHUNK_BYTES // (4 * model.spec.vocab_size))     # (a long text's logits are not held all at once)
+        for first in range(0, len(targets), rows):
+            logits = model.head(h[first:first + rows], ctx.status)
+            parts.append(ops.token_logprobs(logits, tokens[first:first + rows], top=top, status=ctx.status))
+        given, entropy, values, ids = (torch.cat(p).tolist() for p in zip(*parts))
+        return given, entropy, ids, values
 
     @torch.inference_mode()
     def step_and_select(self, entries, sampler, temperatures, keys, positions) -> list:

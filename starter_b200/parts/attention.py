@@ -73,6 +73,8 @@ class GroupedQueryAttention(Part):
         return rotation()
 
     adds_to_stream = True
+    #: a step may bring drafted trees (the parts that cannot see one leave this out)
+    takes_trees = True
 
     def __call__(self, x, ctx, entry, writes_cache=True, add_to=None):
         s = self.spec
@@ -82,7 +84,7 @@ class GroupedQueryAttention(Part):
         qkv = ops.linear(x, weight, status=ctx.status)
         # the position part says what it turns and how; the kernels take or refuse it by name
         cos, sin = ops.rotation_tables(self._rotation(), s.head_dim)
-        if ctx.max_q_len == 1 and ops.decode_from_qkv_takes(s.head_dim, qkv.dtype):
+        if ctx.tree_mask is None and ctx.max_q_len == 1 and ops.decode_from_qkv_takes(s.head_dim, qkv.dtype):
             # one token per sequence: head norm, rotation and cache write inside the attention kernel
             a = ops.attention_decode_qkv(qkv, keys, values, cache.block_table, ctx.seq_slot, ctx.seq_kv_len,
                                          s.num_heads, s.num_kv_heads, s.head_dim, s.scale, s.window,
@@ -94,8 +96,12 @@ class GroupedQueryAttention(Part):
         q = ops.qk_norm_rope_store(
             qkv, s.num_heads, s.num_kv_heads, s.head_dim, self.q_norm, self.k_norm, s.qk_norm_eps,
             cos, sin, ctx.tok_pos, ctx.tok_slot, cache.block_table, keys, values,
-            write_cache=writes_cache)
-        if ctx.max_q_len == 1 and ops.decode_attention_takes(s.head_dim, q.dtype):
+            write_cache=writes_cache, tok_place=ctx.tok_place)
+        if ctx.tree_mask is not None:
+            a = ops.attention_tree(q, keys, values, cache.block_table, ctx.seq_slot, ctx.seq_q_start, ctx.seq_q_len,
+                                   ctx.seq_kv_len, ctx.tok_pos, ctx.tree_mask, s.num_heads, s.num_kv_heads, s.head_dim,
+                                   s.scale, s.window, max_q_len=ctx.max_q_len, kv_hint=ctx.max_kv_len, status=ctx.status)
+        elif ctx.max_q_len == 1 and ops.decode_attention_takes(s.head_dim, q.dtype):
             a = ops.attention_decode(q, keys, values, cache.block_table, ctx.seq_slot, ctx.seq_kv_len,
                                      s.num_heads, s.num_kv_heads, s.head_dim, s.scale, s.window,
                                      status=ctx.status, kv_hint=ctx.max_kv_len)
