@@ -168,36 +168,6 @@ __global__ void __launch_bounds__(TP_WARPS * 32) attention_tree_plain_kernel(con
   }
 }
 
-// Joins the parts of a (node, head): o = sum_s w_s acc_s / sum_s w_s l_s with w_s = 2^(m_s - max m).  A block takes every row of a
-// sequence's node, a warp a head at a time.
-template <typename T>
-__global__ void attention_tree_join_kernel(const TreeArgs a) {
-  pdl_trigger();
-  pdl_wait();
-  const int seq = blockIdx.y, node = blockIdx.x;
-  if (node >= a.seq_q_len[seq]) return;
-  const int lane = threadIdx.x & 31;
-  const float* part_ml = a.part_ml;
-  const float* part_acc = a.part_acc;
-  SB_BEHIND_WAIT(part_ml);
-  SB_BEHIND_WAIT(part_acc);
-  for (int h = threadIdx.x >> 5; h < a.heads; h += blockDim.x >> 5) {
-    const size_t at = (size_t)(a.seq_q_start[seq] + node) * a.heads + h, p0 = at * a.splits;
-    float top = -INFINITY, sum = 0.f;
-    for (int s = 0; s < a.splits; ++s)
-      if (part_ml[2 * (p0 + s) + 1] != 0.f) top = fmaxf(top, part_ml[2 * (p0 + s)]);
-    for (int s = 0; s < a.splits; ++s)
-      if (part_ml[2 * (p0 + s) + 1] != 0.f) sum = fmaf(part_ml[2 * (p0 + s) + 1], exp2f(part_ml[2 * (p0 + s)] - top), sum);
-    const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
-    for (int d = lane; d < a.dim; d += 32) {
-      float o = 0.f;
-      for (int s = 0; s < a.splits; ++s)
-        if (part_ml[2 * (p0 + s) + 1] != 0.f) o = fmaf(part_acc[(p0 + s) * a.dim + d], exp2f(part_ml[2 * (p0 + s)] - top), o);
-      ((T*)a.out)[at * a.dim + d] = from_f<T>(o * inv);
-    }
-  }
-}
-
 template <typename T, int NI>
 static int launch_plain(const TreeArgs& a, int seqs, int max_q_len, cudaStream_t s) {
   const int pitch = ((a.dim + 3) & ~3) + 4, smem = (TP_TILE + 2 * TP_KEYS) * pitch * 4;
@@ -210,18 +180,18 @@ static int launch_plain(const TreeArgs& a, int seqs, int max_q_len, cudaStream_t
   const dim3 grid((max_q_len * (a.heads / a.kv_heads) + TP_TILE - 1) / TP_TILE, a.kv_heads, seqs * a.splits);
   int rc = launch_dependent(attention_tree_plain_kernel<T, NI>, grid, dim3(TP_WARPS * 32), smem, s, a, wide);
   if (rc || a.splits == 1) return rc;
-  return launch_dependent(attention_tree_join_kernel<T>, dim3(max_q_len, seqs), dim3(128), 0, s, a);
+  return launch_dependent(attention_tree_join_kernel<T>, dim3(max_q_len, seqs, (a.heads + 3) / 4), dim3(128), 0, s, a);
 }
 
 extern "C" {
 
-// dtype 0 float, 1 bfloat16; dim up to 256; splits from 1 on, with part_acc and part_ml (see TreeArgs) from 2 on.
+// dtype 0 float, 1 bfloat16; dim up to 256; splits 1 to 32, with part_acc and part_ml (see TreeArgs) from 2 on.
 int sb_attention_tree_plain(int dtype, const void* q, void* out, const void* k_store, const void* v_store, const int* block_table,
                             int table_stride, const int* seq_slot, const int* seq_q_start, const int* seq_q_len, const int* seq_kv_len,
                             const int* tok_pos, const void* mask, int words, int seqs, int max_q_len, int heads, int kv_heads, int dim,
                             float scale, int window, int splits, float* part_acc, float* part_ml, cudaStream_t s) {
   if (seqs == 0 || max_q_len == 0) return 0;
-  if (kv_heads <= 0 || heads % kv_heads || dim < 1 || dim > 256 || words < 1 || splits < 1) return -2;
+  if (kv_heads <= 0 || heads % kv_heads || dim < 1 || dim > 256 || words < 1 || splits < 1 || splits > 32) return -2;
   if ((long long)seqs * splits > 65535 || kv_heads > 65535 || seqs > 65535) return -2;
   if (splits > 1 && (!part_acc || !part_ml)) return -2;
   const TreeArgs a{q, out, k_store, v_store, block_table, table_stride, seq_slot, seq_q_start, seq_q_len, seq_kv_len, tok_pos,

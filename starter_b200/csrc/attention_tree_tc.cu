@@ -1,0 +1,563 @@
+// Attention of the nodes of drafted trees over the paged cache (see attention_tree.cuh) on the fifth-generation tensor cores, in bfloat16:
+// steps whose trees have many rows.
+//
+// A block takes 256 packed rows of one key/value head as two tiles of 128 and walks the sequence's keys in steps of 128 (two pages):
+//     S  = Q K^T     M = 128 rows, N = 128 keys,  K = head_dim        (Q and K K-major)
+//     O += P V       M = 128 rows, N = head_dim,  K = 128 keys        (V as it lies in the cache, "MN-major")
+// with S and O of both tiles in tensor memory.  Warps 0-3 and 4-7 are the softmax of tile 0 and 1 (thread = row = tensor-memory lane), warp 8
+// brings keys and values by TMA, warps 9 and 10 issue the products of tile 0 and 1: the schedule of the prompt attention
+// (attention_prefill_tc.cu), with all of a sequence's trees' rows on one copy of its keys.  The queries of a tile lie in up to 128 pieces of
+// the packed rows; every softmax thread puts its own row into shared memory.
+//
+// A row's view of a page is 64 bits: ones for what is cached (from its window's first place on), then the bits of its mask, shifted to where
+// the nodes begin in the page.  Only pages that some row does not see whole are masked.  On those a value that is no number is taken out of
+// the tile before its product (it must not reach rows that do not see it, though their weight is zero) and put onto the results of the rows
+// that see it at the end.
+//
+// Few blocks over many keys: `splits` CTAs, a cluster, walk a part of a block's keys each and meet through distributed shared memory.
+// Every wait on an mbarrier gives up after WAIT_LIMIT_NS, raises bit 16 of *status and lets the block drain its copies, free its tensor memory
+// and return.
+#include <cuda.h>
+
+#include "attention_tc.cuh"
+#include "attention_tree.cuh"
+#include "tensor_map.cuh"
+
+#define TT_BK 128
+#define TT_THREADS 352
+#define TT_ROWS (2 * TC_BQ)
+#define TT_MAX_NODES 256
+#define TT_MAX_SPLITS 8
+
+#define TT_WORDS (TT_MAX_NODES / 32)
+// Places j0 .. j0 + 63 as the row sees them: bits[] is its mask, `first` its window's first place (0: no window).
+__device__ __forceinline__ uint64_t tt_view(const uint32_t* bits, int first, int past, int q_len, int j0) {
+  uint64_t view = 0;
+#pragma unroll
+  for (int w = 0; w < TT_WORDS; ++w) {                    // (every word by its number, so that they stay in registers)
+    const int at = past + 32 * w - j0;                    // where its first node stands in the page
+    if (at > -32 && at < 64) view |= at >= 0 ? (uint64_t)bits[w] << at : (uint64_t)(bits[w] >> -at);
+  }
+  const int cached = past - j0, end = cached + q_len, hidden = min(first, past) - j0;
+  if (cached > 0) view |= cached < 64 ? (1ull << cached) - 1 : ~0ull;
+  if (end < 64) view &= end > 0 ? (1ull << end) - 1 : 0ull;          // places behind the sequence
+  if (hidden > 0) view &= hidden < 64 ? ~0ull << hidden : 0ull;      // cached places in front of the window
+  return view;
+}
+__device__ __forceinline__ bool tt_no_number(uint32_t half) { return (half & 0x7f80u) == 0x7f80u; }
+
+// DC: 64-element (128-byte) chunks of a head.
+template <int DC, bool PARTS>
+__global__ void __launch_bounds__(TT_THREADS, 1)
+attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const TreeArgs a, int* status) {
+  constexpr int D = DC * 64;
+  constexpr int SUB = 128 * 128;                          // bytes of a [128 rows x 128 bytes] sub-tile
+  constexpr int Q_BYTES = DC * SUB, KV_BYTES = DC * SUB, P_BYTES = 2 * SUB;
+  constexpr uint32_t TMEM_COLS = 512;                     // S of both tiles: 2 x 128; O of both tiles: 2 x 128
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint8_t* q_sm = smem;                                   // 2 tiles
+  uint8_t* p_sm = q_sm + 2 * Q_BYTES;                     // 2 tiles
+  uint8_t* ring = p_sm + 2 * P_BYTES;                     // buffers 0 and 1: keys of even and odd steps; 2: values
+  __shared__ uint64_t q_ready[2], full[3], empty[3], s_ready[2], s_free[2], p_ready[2], o_ready[2];
+  __shared__ uint32_t tmem_holder;
+  __shared__ int abort_flag, sh_low, sh_high, sh_bad;
+  float2 row_state = make_float2(-INFINITY, 0.f);         // keys in parts: a row's reference and sum
+
+  pdl_trigger();
+  pdl_wait();
+  const int splits = PARTS ? a.splits : 1, block = blockIdx.x / splits, part = blockIdx.x - block * splits;
+  const int seq = blockIdx.y / a.kv_heads, kvh = blockIdx.y - seq * a.kv_heads;
+  const int q_len = min(a.seq_q_len[seq], TT_MAX_NODES), kv_len = a.seq_kv_len[seq], past = kv_len - q_len, start = a.seq_q_start[seq];
+  const int group = a.heads / a.kv_heads, row0 = block * TT_ROWS, n_rows = q_len * group;
+  if (row0 >= n_rows) return;                             // (the same in every block of a cluster)
+  const int rows_valid = min(TT_ROWS, n_rows - row0), tiles = rows_valid > TC_BQ ? 2 : 1;
+  const int node0 = row0 / group, n_nodes = (row0 + rows_valid - 1) / group - node0 + 1;
+  const int* pages = a.block_table + (size_t)a.seq_slot[seq] * a.table_stride;
+  // the warp's number as a value the compiler knows to be the same in every lane
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < 3; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], tiles); }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&q_ready[t], 4);                          // one arrival per softmax warp
+      mbar_init(&s_ready[t], 1);
+      mbar_init(&s_free[t], 4);
+      mbar_init(&p_ready[t], 4);
+      mbar_init(&o_ready[t], 1);
+    }
+    abort_flag = 0;
+    sh_low = a.window > 0 ? past : 0;
+    sh_high = 0;
+    sh_bad = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 9) tmem_alloc(&tmem_holder, TMEM_COLS);
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem_base = tmem_holder;
+  if (a.window > 0) {
+    for (int n = threadIdx.x; n < n_nodes; n += TT_THREADS) {
+      const int first = a.tok_pos[start + node0 + n] - a.window + 1;
+      atomicMin(&sh_low, max(first, 0));                  // the first place any row sees
+      atomicMax(&sh_high, min(first, past));              // from here on every row sees all that is cached
+    }
+    __syncthreads();
+  }
+  const int page_lo = sh_low / SB_PAGE_TOKENS, page_hi = (kv_len - 1) / SB_PAGE_TOKENS, high = sh_high;
+  int n_steps = (page_hi - page_lo) / 2 + 1, first_step = 0;
+  if constexpr (PARTS) {                                  // this CTA's steps
+    const int per = (n_steps + splits - 1) / splits;
+    first_step = part * per;
+    n_steps = max(0, min(per, n_steps - first_step));
+  }
+  volatile int* abort = &abort_flag;
+
+  if (warp == 8) {
+    // ---------------- producer: the whole warp walks the schedule, one elected lane issues the copies
+    const bool elected = elect_one();
+    // Keys alternate between buffers 0 and 1 and run a step ahead of the values, which have buffer 2: K0 V0 K1 | K2 V1 | K3 V2 ...
+    auto load = [&](bool is_v, int i) -> bool {
+      const int b = is_v ? 2 : (i & 1), use = is_v ? i : (i >> 1);
+      if (use > 0 && !__all_sync(0xffffffffu, mbar_wait(&empty[b], (use - 1) & 1, abort))) return false;
+      if (elected) mbar_expect_tx(&full[b], DC * SUB);
+      const bool withheld = is_v && first_step + i == *(volatile int*)&tc_withhold_step;   // tests only
+      for (int half = 0; half < (withheld ? 1 : 2); ++half) {
+        const int row = (pages[min(page_lo + 2 * (first_step + i) + half, page_hi)] * a.kv_heads + kvh) * SB_PAGE_TOKENS;
+        for (int c = 0; c < DC; ++c)
+          if (elected) tma_load_2d(ring + b * KV_BYTES + c * SUB + half * 8192, is_v ? &map_v : &map_k, &full[b], c * 64, row);
+      }
+      return true;
+    };
+    int loads[3] = {0, 0, 0};                             // per buffer: how many copies were started
+    bool ok = n_steps > 0 && load(false, 0);
+    if (ok) { loads[0]++; ok = load(true, 0); }
+    if (ok) loads[2]++;
+    if (ok && n_steps > 1) { ok = load(false, 1); if (ok) loads[1]++; }
+    for (int i = 1; i < n_steps && ok; ++i) {
+      if (i + 1 < n_steps) { ok = load(false, i + 1); if (ok) loads[(i + 1) & 1]++; }
+      if (ok) { ok = load(true, i); if (ok) loads[2]++; }
+    }
+    if (*abort && elected) {                              // let the copies in flight land before the block ends
+      for (int b = 0; b < 3; ++b) {
+        const uint64_t begun = now_ns();
+        while (loads[b] > 0 && !mbar_try(&full[b], (loads[b] - 1) & 1) && now_ns() - begun < WAIT_LIMIT_NS) {}
+      }
+    }
+  } else if (warp == 9 || warp == 10) {
+    // ---------------- MMA issuers: warp 9 for tile 0, warp 10 for tile 1, each with its own chain of waits
+    const int t = warp - 9;
+    if (t < tiles && n_steps > 0) {
+      const bool elected = elect_one();
+      const uint32_t idesc_s = instr_desc(TT_BK, 0), idesc_o = instr_desc(D, 1);
+      const uint32_t q_addr = smem_u32(q_sm + t * Q_BYTES), p_addr = smem_u32(p_sm + t * P_BYTES);
+      auto issue_s = [&](int buf) {
+        if (elected) {
+#pragma unroll
+          for (int k = 0; k < DC * 4; ++k) {
+            const uint32_t off = (k >> 2) * SUB + (k & 3) * 32;
+            umma_bf16(tmem_base + t * TT_BK, smem_desc(q_addr + off, 16), smem_desc(smem_u32(ring + buf * KV_BYTES) + off, 16), idesc_s,
+                      k > 0 ? 1u : 0u);
+          }
+          umma_commit(&s_ready[t]);
+          umma_commit(&empty[buf]);
+        }
+        __syncwarp();
+      };
+      auto issue_pv = [&](bool first) {
+        if (elected) {
+#pragma unroll
+          for (int k = 0; k < TT_BK / 16; ++k)
+            umma_bf16(tmem_base + 2 * TT_BK + t * 128, smem_desc(p_addr + (k >> 2) * SUB + (k & 3) * 32, 16),
+                      smem_desc(smem_u32(ring + 2 * KV_BYTES) + k * 2048, SUB), idesc_o, (first && k == 0) ? 0u : 1u);
+          umma_commit(&o_ready[t]);
+          umma_commit(&empty[2]);
+        }
+        __syncwarp();
+      };
+      // every lane waits; the warp goes on together or stops together
+      auto wait2 = [&](uint64_t* first_bar, uint32_t first_parity, uint64_t* second_bar, uint32_t second_parity) -> bool {
+        const bool got = mbar_wait(first_bar, first_parity, abort) && mbar_wait(second_bar, second_parity, abort);
+        return __all_sync(0xffffffffu, got);
+      };
+      bool ok = wait2(&q_ready[t], 0, &full[0], 0);
+      if (ok) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        issue_s(0);
+      }
+      // Step i: S of step i+1 as soon as the softmax warps have read S of step i out of tensor memory, then PV of step i when P is written.
+      for (int i = 0; i < n_steps && ok; ++i) {
+        if (i + 1 < n_steps) {
+          const int kb = (i + 1) & 1;                     // buffer of K(i+1); V(i) is in buffer 2
+          ok = wait2(&full[kb], ((i + 1) >> 1) & 1, &s_free[t], i & 1);
+          if (!ok) break;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          issue_s(kb);
+        }
+        ok = wait2(&full[2], i & 1, &p_ready[t], i & 1);
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        issue_pv(i == 0);
+      }
+    }
+  } else if (warp < 8 && (warp >> 2) < tiles) {
+    // ---------------- softmax and output: thread = packed row = tensor-memory lane.  The running output stays in tensor memory and is rescaled
+    // only when a row's maximum has outgrown the reference by more than 2^8, so most steps only produce P.
+    const int t = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
+    const int row = row0 + min(t * TC_BQ + r, rows_valid - 1), node = row / group;   // (rows behind the last look like the last)
+    const bool valid = t * TC_BQ + r < rows_valid;
+    const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
+    const uint32_t tmem_s = tmem_base + t * TT_BK + lane_addr, tmem_o = tmem_base + 2 * TT_BK + t * 128 + lane_addr;
+    uint8_t* p_row = p_sm + t * P_BYTES + r * 128;
+    const size_t at = ((size_t)(start + node) * a.heads + kvh * group + row % group) * D;
+    {
+      // K-major A operand: 64-element chunk dc, 16-byte column c ^ (r % 8) of row r
+      const uint4* src = reinterpret_cast<const uint4*>((const bf16*)a.q + at);
+      uint4 v[8];
+#pragma unroll
+      for (int dc = 0; dc < DC; ++dc) {
+#pragma unroll
+        for (int c = 0; c < 8; ++c) v[c] = src[dc * 8 + c];
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+          *reinterpret_cast<uint4*>(q_sm + t * Q_BYTES + dc * SUB + r * 128 + ((c ^ (r & 7)) << 4)) = v[c];
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_ready[t]);
+    }
+    const int first = a.window > 0 ? a.tok_pos[start + node] - a.window + 1 : 0;
+    uint32_t bits[TT_WORDS];
+#pragma unroll
+    for (int w = 0; w < TT_WORDS; ++w) {
+      bits[w] = w < a.words ? a.mask[(size_t)(start + node) * a.words + w] : 0u;
+      if (a.window > 0) {                                 // without the nodes in front of the window
+        for (uint32_t left = bits[w]; left; left &= left - 1) {
+          const int m = 32 * w + __ffs(left) - 1;
+          if (m >= q_len || a.tok_pos[start + m] < first) bits[w] &= ~(left & -left);
+        }
+      }
+    }
+    float m_ref = -INFINITY, l_run = 0.f;
+    bool ok = true;
+    // the whole warp goes on or the whole warp stops: tensor memory is read and written by warps
+    auto together = [&](bool got) -> bool { return __all_sync(0xffffffffu, got); };
+    for (int i = 0; i < n_steps && ok; ++i) {
+      const int j0 = (page_lo + 2 * (first_step + i)) * SB_PAGE_TOKENS;
+      const bool edge = j0 + TT_BK > past || j0 < high;   // some row does not see all of the step
+      if (edge) {
+        // values that are no numbers leave the tile (both tiles' warps may find the same: they write the same zeros).  These warps may be a
+        // step ahead of the values: only behind PV of the step before does the barrier's parity speak of this step's.
+        ok = together((i == 0 || mbar_wait(&o_ready[t], (i - 1) & 1, abort)) && mbar_wait(&full[2], i & 1, abort));
+        if (!ok) break;
+        int bad = 0;
+        uint4* v = reinterpret_cast<uint4*>(ring + 2 * KV_BYTES);
+#pragma unroll 4
+        for (int idx = (warp & 3) * 32 + lane; idx < DC * SUB / 16; idx += 128) {
+          const uint4 x = v[idx];
+          uint32_t w[4] = {x.x, x.y, x.z, x.w};
+          int here = 0;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if (tt_no_number(w[e])) { w[e] &= 0xffff0000u; here = 1; }
+            if (tt_no_number(w[e] >> 16)) { w[e] &= 0xffffu; here = 1; }
+          }
+          if (here) { v[idx] = make_uint4(w[0], w[1], w[2], w[3]); bad = 1; }
+        }
+        if (bad) sh_bad = 1;
+      }
+      ok = together(mbar_wait(&s_ready[t], i & 1, abort));
+      if (!ok) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      float sv[64];
+      float rs = 0.f, rs_hi = 0.f;                        // the row sum in two halves (packed adds)
+      // half h of the row of S from tensor memory, masked where the step touches an edge
+      auto load_half = [&](int h) {
+        tmem_load64(tmem_s + h * 64, sv);
+        if (edge) {
+          const uint64_t view = tt_view(bits, first, past, q_len, j0 + h * 64);
+          const uint32_t lo = (uint32_t)view, hi = (uint32_t)(view >> 32);
+#pragma unroll
+          for (int e = 0; e < 64; ++e)
+            if (!((e < 32 ? lo >> e : hi >> (e - 32)) & 1u)) sv[e] = -INFINITY;
+        }
+      };
+      uint32_t pk[32];
+      float mx = -INFINITY, m_use = m_ref == -INFINITY ? 0.f : m_ref;
+      // P = exp2(S * scale - m) of 8 keys, rounded to bfloat16: one 16-byte column of the A operand
+      auto exp8 = [&](int c, uint32_t* w) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float x0, x1;
+          fma2(x0, x1, sv[c * 8 + 2 * e], sv[c * 8 + 2 * e + 1], a.scale_log2, -m_use);
+          const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
+          add2(rs, rs_hi, p0, p1);
+          const __nv_bfloat162 two = __floats2bfloat162_rn(p0, p1);
+          w[e] = *reinterpret_cast<const uint32_t*>(&two);
+        }
+      };
+      auto store8 = [&](int h, int c, const uint32_t* w) {
+        *reinterpret_cast<uint4*>(p_row + h * SUB + ((c ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+      };
+      auto s_consumed = [&]() {                           // S of this step may be overwritten
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_free[t]);
+      };
+      // One pass in the common case: the exponent's reference is the one of the step before.
+      load_half(0);
+#pragma unroll
+      for (int e = 0; e < 64; ++e) mx = fmaxf(mx, sv[e]);
+#pragma unroll
+      for (int c = 0; c < 8; ++c) exp8(c, pk + 4 * c);
+      load_half(1);
+#pragma unroll
+      for (int e = 0; e < 64; ++e) mx = fmaxf(mx, sv[e]);
+      mx *= a.scale_log2;                                 // scale_log2 > 0: the maximum commutes with it
+      const bool outgrown = mx > m_ref + 8.f;             // also the first keys a row sees (m_ref = -inf)
+      if (!__any_sync(0xffffffffu, outgrown)) {
+        s_consumed();
+        // P's tile and O are free once PV of the step before has finished
+        if (i > 0) ok = together(mbar_wait(&o_ready[t], (i - 1) & 1, abort));
+        if (!ok) break;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) store8(0, c, pk + 4 * c);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          uint32_t w[4];
+          exp8(c, w);
+          store8(1, c, w);
+        }
+      } else {
+        // a new reference: rescale what has been accumulated, then redo this step's P
+        const float m_new = fmaxf(m_ref, mx);
+        const float alpha = m_ref == -INFINITY ? 1.f : fast_exp2(m_ref - m_new);
+        if (i > 0) {
+          ok = together(mbar_wait(&o_ready[t], (i - 1) & 1, abort));
+          if (!ok) break;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll 1
+          for (int c = 0; c < D; c += 32) {
+            float ov[32];
+            tmem_load32(tmem_o + c, ov);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) ov[e] *= alpha;
+            tmem_store32(tmem_o + c, ov);
+          }
+          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        }
+        l_run *= alpha;
+        m_ref = m_new;
+        m_use = m_ref == -INFINITY ? 0.f : m_ref;
+        rs = 0.f;
+        rs_hi = 0.f;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          uint32_t w[4];
+          exp8(c, w);
+          store8(1, c, w);
+        }
+        load_half(0);
+        s_consumed();
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          uint32_t w[4];
+          exp8(c, w);
+          store8(0, c, w);
+        }
+      }
+      l_run += rs + rs_hi;
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_ready[t]);
+    }
+    if (ok && n_steps > 0) ok = together(mbar_wait(&o_ready[t], (n_steps - 1) & 1, abort));
+    if (ok && n_steps > 0) {
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const bool bad = *(volatile int*)&sh_bad != 0;
+      if constexpr (PARTS) row_state = make_float2(m_ref, l_run);
+      const float inv = l_run > 0.f ? 1.f / l_run : l_run == 0.f ? 0.f : l_run;
+      bf16* dst = (bf16*)a.out + at;
+#pragma unroll 1
+      for (int c = 0; c < D; c += 32) {
+        float ov[32];
+        tmem_load32(tmem_o + c, ov);
+        if (bad) {                                        // what was taken out of the tiles, to the rows that see it
+          const int last = min((page_lo + 2 * (first_step + n_steps)) * SB_PAGE_TOKENS, kv_len);
+          for (int j = (page_lo + 2 * first_step) * SB_PAGE_TOKENS; j < last; ++j) {
+            if (!(tt_view(bits, first, past, q_len, j) & 1ull)) continue;
+            const bf16* v = (const bf16*)a.v_store + page_row(pages[j / SB_PAGE_TOKENS], kvh, j % SB_PAGE_TOKENS, a.kv_heads, D) + c;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              const float x = __bfloat162float(v[e]);
+              if (!(fabsf(x) < INFINITY)) ov[e] += x;
+            }
+          }
+        }
+        if constexpr (PARTS) {
+#pragma unroll
+          for (int d = 0; d < 32; d += 4)
+            *reinterpret_cast<float4*>(part_piece<64, D>(p_sm + t * P_BYTES, q_sm + t * Q_BYTES, r, (c + d) / 4)) =
+                make_float4(ov[d], ov[d + 1], ov[d + 2], ov[d + 3]);
+        } else if (valid) {
+#pragma unroll
+          for (int d = 0; d < 32; d += 8) {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const __nv_bfloat162 two = __floats2bfloat162_rn(ov[d + 2 * e] * inv, ov[d + 2 * e + 1] * inv);
+              w[e] = *reinterpret_cast<const uint32_t*>(&two);
+            }
+            *reinterpret_cast<uint4*>(dst + c + d) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+      }
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    }
+  }
+
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  if constexpr (PARTS) {
+    // (the rows' states lie where keys were: both tiles are done with them behind the block's barrier)
+    float2* ml = reinterpret_cast<float2*>(ring);
+    __syncthreads();
+    if (threadIdx.x < TT_ROWS) ml[threadIdx.x] = row_state;
+    cluster_barrier();
+    // every CTA joins its share of the rows: 16 threads a row, D / 16 columns each
+    const int share = (rows_valid + splits - 1) / splits, c = (threadIdx.x & 15) * (D / 16);
+    if (threadIdx.x < TT_ROWS) {
+      for (int n = threadIdx.x >> 4; n < share; n += TT_ROWS / 16) {
+        const int mine = part * share + n;
+        if (mine >= rows_valid) break;
+        const int t = mine / TC_BQ, r = mine % TC_BQ;
+        float2 ps[TT_MAX_SPLITS];
+        float top = -INFINITY, sum = 0.f, o[D / 16];
+#pragma unroll
+        for (int p = 0; p < TT_MAX_SPLITS; ++p) {
+          ps[p] = p < splits ? peer_load2(peer_u32(ml + mine, p)) : make_float2(-INFINITY, 0.f);
+          if (ps[p].y != 0.f) top = fmaxf(top, ps[p].x);
+        }
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) o[d] = 0.f;
+#pragma unroll
+        for (int p = 0; p < TT_MAX_SPLITS; ++p) {
+          // (a part without keys filed nothing; one whose sum is no number has a score that is none, which is the row's result)
+          if (p >= splits || ps[p].y == 0.f) continue;
+          const float w = fast_exp2(ps[p].x - top);
+          sum = fmaf(w, ps[p].y, sum);
+#pragma unroll
+          for (int d = 0; d < D / 16; d += 4) {
+            const float4 x = peer_load4(peer_u32(part_piece<64, D>(p_sm + t * P_BYTES, q_sm + t * Q_BYTES, r, (c + d) / 4), p));
+            o[d] = fmaf(w, x.x, o[d]); o[d + 1] = fmaf(w, x.y, o[d + 1]); o[d + 2] = fmaf(w, x.z, o[d + 2]); o[d + 3] = fmaf(w, x.w, o[d + 3]);
+          }
+        }
+        const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
+        const int row = row0 + mine;
+        bf16* dst = (bf16*)a.out + ((size_t)(start + row / group) * a.heads + kvh * group + row % group) * D + c;
+#pragma unroll
+        for (int d = 0; d < D / 16; d += 4) {
+          const __nv_bfloat162 two = __floats2bfloat162_rn(o[d] * inv, o[d + 1] * inv), more = __floats2bfloat162_rn(o[d + 2] * inv, o[d + 3] * inv);
+          *reinterpret_cast<uint2*>(dst + d) = make_uint2(*reinterpret_cast<const uint32_t*>(&two), *reinterpret_cast<const uint32_t*>(&more));
+        }
+      }
+    }
+    cluster_barrier();                                    // nobody leaves while others read from it
+  }
+  __syncthreads();
+  if (warp == 9) {
+    __syncwarp();
+    tmem_free(tmem_holder, TMEM_COLS);
+  }
+  if (threadIdx.x == 0 && abort_flag && status) atomicOr(status, 16);
+}
+
+// ------------------------------------------------------------------------------------------ host
+
+template <int DC> static constexpr int tt_smem() { return (2 * DC + 4 + 3 * DC) * 128 * 128 + 1024; }
+
+template <int DC, bool PARTS>
+static int launch_as(const CUtensorMap& mk, const CUtensorMap& mv, const TreeArgs& a, int seqs, int max_q_len, int* status, cudaStream_t s) {
+  // (an attribute of the device the launch goes to)
+  const cudaError_t e = cudaFuncSetAttribute(attention_tree_tc_kernel<DC, PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, tt_smem<DC>());
+  if (e != cudaSuccess) return (int)e;
+  const int blocks = (max_q_len * (a.heads / a.kv_heads) + TT_ROWS - 1) / TT_ROWS;
+  const dim3 grid(blocks * a.splits, seqs * a.kv_heads);
+  if (PARTS) return launch_dependent_cluster(attention_tree_tc_kernel<DC, PARTS>, grid, dim3(TT_THREADS), tt_smem<DC>(), s, dim3(a.splits), mk, mv, a, status);
+  return launch_dependent(attention_tree_tc_kernel<DC, PARTS>, grid, dim3(TT_THREADS), tt_smem<DC>(), s, mk, mv, a, status);
+}
+
+static unsigned long long next_limit_ns = WAIT_LIMIT_NS;
+static int next_withhold_step = -1;
+
+extern "C" {
+
+// For tests of the give-up path: the NEXT sb_attention_tree_tc launch leaves out half of the values of step `step` (128 keys) of every block
+// and its waits give up after `limit_ns`.  The blocks cannot finish; the launch must return with bit 16 of *status set.
+void sb_attention_tree_tc_withhold(int step, unsigned long long limit_ns) {
+  next_withhold_step = step;
+  next_limit_ns = limit_ns ? limit_ns : WAIT_LIMIT_NS;
+}
+
+// How many clusters of `size` of its CTAs, which take an SM each, the current device runs at once, or minus an error.
+int sb_attention_tree_tc_clusters(int size) {
+  auto kernel = attention_tree_tc_kernel<2, true>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, tt_smem<2>());
+  if (e != cudaSuccess) return -(int)e;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = size;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(size);
+  cfg.blockDim = dim3(TT_THREADS);
+  cfg.dynamicSmemBytes = tt_smem<2>();
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
+  return e == cudaSuccess ? n : -(int)e;
+}
+
+// bfloat16, dim 64 or 128 (-2 otherwise), scale > 0, q, out and the stores 16-byte aligned; splits 1, 2, 4 or 8; n_pages: pages in the stores.
+int sb_attention_tree_tc(const void* q, void* out, const void* k_store, const void* v_store, int n_pages, const int* block_table,
+                         int table_stride, const int* seq_slot, const int* seq_q_start, const int* seq_q_len, const int* seq_kv_len,
+                         const int* tok_pos, const void* mask, int words, int seqs, int max_q_len, int heads, int kv_heads, int dim,
+                         float scale, int window, int splits, int* status, cudaStream_t s) {
+  if (seqs == 0 || max_q_len == 0) return 0;
+  if (kv_heads <= 0 || heads % kv_heads || words < 1 || !(scale > 0.f) || max_q_len > TT_MAX_NODES) return -2;
+  if ((dim != 64 && dim != 128) || (splits != 1 && splits != 2 && splits != 4 && splits != TT_MAX_SPLITS)) return -2;
+  if ((long long)seqs * kv_heads > 65535) return -2;
+  if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_store | (uintptr_t)v_store) & 15) return -2;
+  // (a TMA coordinate is 32 bits)
+  const long long kv_rows = (long long)n_pages * kv_heads * SB_PAGE_TOKENS;
+  if (kv_rows > 0x7fffffffll) return -2;
+  CUtensorMap mk, mv;
+  int rc = sb_make_map(&mk, k_store, kv_rows, dim, SB_PAGE_TOKENS);
+  if (rc) return rc;
+  rc = sb_make_map(&mv, v_store, kv_rows, dim, SB_PAGE_TOKENS);
+  if (rc) return rc;
+  const TreeArgs a{q, out, k_store, v_store, block_table, table_stride, seq_slot, seq_q_start, seq_q_len, seq_kv_len, tok_pos,
+                   (const uint32_t*)mask, words < TT_MAX_NODES / 32 ? words : TT_MAX_NODES / 32, heads, kv_heads, dim,
+                   scale * 1.4426950408889634f, window > 0 ? window : 0, splits, nullptr, nullptr};
+  const bool test_run = next_withhold_step >= 0;
+  if (test_run) {
+    cudaMemcpyToSymbolAsync(tc_withhold_step, &next_withhold_step, sizeof(int), 0, cudaMemcpyHostToDevice, s);
+    cudaMemcpyToSymbolAsync(tc_wait_limit_ns, &next_limit_ns, sizeof(next_limit_ns), 0, cudaMemcpyHostToDevice, s);
+    cudaStreamSynchronize(s);
+  }
+  if (dim == 64) rc = splits > 1 ? launch_as<1, true>(mk, mv, a, seqs, max_q_len, status, s) : launch_as<1, false>(mk, mv, a, seqs, max_q_len, status, s);
+  else rc = splits > 1 ? launch_as<2, true>(mk, mv, a, seqs, max_q_len, status, s) : launch_as<2, false>(mk, mv, a, seqs, max_q_len, status, s);
+  if (test_run) {
+    cudaStreamSynchronize(s);
+    next_withhold_step = -1;
+    next_limit_ns = WAIT_LIMIT_NS;
+    cudaMemcpyToSymbolAsync(tc_withhold_step, &next_withhold_step, sizeof(int), 0, cudaMemcpyHostToDevice, s);
+    cudaMemcpyToSymbolAsync(tc_wait_limit_ns, &next_limit_ns, sizeof(next_limit_ns), 0, cudaMemcpyHostToDevice, s);
+    cudaStreamSynchronize(s);
+  }
+  return rc;
+}
+
+}  // extern "C"

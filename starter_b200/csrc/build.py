@@ -67,6 +67,8 @@ SOURCES = (
     "state_scan_prompt",
     "state_step",
     "attention_tree",
+    "attention_tree_mma",
+    "attention_tree_tc",
     "cache_pages",
     "token_logprobs",
 )

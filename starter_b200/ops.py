@@ -1329,8 +1329,30 @@ def _tree_plain_splits(blocks: int, keys: int) -> int:
     return max(1, min(-(-keys // 64), 592 // max(blocks, 1), 32))
 
 
+@functools.lru_cache(maxsize=4096)
+def _tree_mma_plan(rows: int, units: int, keys: int) -> tuple:
+    """``(row warps, splits)`` of the mma.sync kernel for ``rows`` packed rows of each of ``units`` (sequence, key/value head) pairs."""
+    row_warps = 1 if rows <= 16 else 2 if rows <= 32 else 4
+    blocks = units * -(-rows // (16 * row_warps))
+    return row_warps, max(1, min(8, (2 * SM_COUNT) // blocks, -(-keys // PAGE_TOKENS)))
+
+
+@functools.lru_cache(maxsize=None)
+def _tree_tc_clusters(size: int, device: int) -> int:
+    got = _lib("attention_tree_tc").sb_attention_tree_tc_clusters(size)
+    if got < 0:
+        raise KernelError(f"the device does not say how many clusters of {size} it runs at once (CUDA error {-got})")
+    return got
+
+
+def _tree_tc_splits(blocks: int, keys: int, device: int) -> int:
+    """How many CTAs share the keys of a block of 256 rows: as many as run at once."""
+    return next((parts for parts in (8, 4, 2) if keys >= 256 * parts and blocks <= _tree_tc_clusters(parts, device)), 1)
+
+
 def attention_tree(q, k_store, v_store, block_table, seq_slot, seq_q_start, seq_q_len, seq_kv_len, tok_pos, tree_mask, heads, kv_heads,
-                   head_dim, scale, window=None, max_q_len=None, kv_hint=0, status=None):
+                   head_dim, scale, window=None, max_q_len=None, kv_hint=0, status=None, kernel=None, parts=None,
+                   withhold=None):
     """Attention of the nodes of drafted trees over the paged cache.
 
     ``q`` ``[T, heads * head_dim]`` packed by sequence; the ``seq_*`` arrays describe each sequence of the step as they do for
@@ -1370,7 +1392,37 @@ def attention_tree(q, k_store, v_store, block_table, seq_slot, seq_q_start, seq_
     if q.shape[0] == 0 or seqs == 0:
         return out
     group = heads // kv_heads
-    splits = _tree_plain_splits(-(-max_q_len * group // 16) * kv_heads * seqs, min(kv_hint, window + max_q_len) if window else kv_hint)
+    aligned = code == 1 and not (q.data_ptr() | k_store.data_ptr() | v_store.data_ptr()) & 15
+    keys = min(kv_hint, window + max_q_len) if window else kv_hint
+    if kernel is None:
+        kernel = "plain" if not aligned or head_dim not in PREFILL_HEAD_DIMS else "mma"
+        if (kernel == "mma" and head_dim in PREFILL_TC_HEAD_DIMS and scale > 0 and max_q_len * group > 64
+                and k_store.shape[0] * kv_heads * PAGE_TOKENS < 1 << 31):
+            kernel = "tcgen05"
+    if kernel == "tcgen05":
+        if withhold is not None:
+            _lib("attention_tree_tc").sb_attention_tree_tc_withhold(int(withhold[0]), int(withhold[1]))
+        splits = parts or _tree_tc_splits(-(-max_q_len * group // 256) * kv_heads * seqs, keys, q.get_device())
+        rc = _lib("attention_tree_tc").sb_attention_tree_tc(
+            q, out, k_store, v_store, k_store.shape[0], block_table, block_table.shape[1], seq_slot, seq_q_start, seq_q_len, seq_kv_len,
+            tok_pos, tree_mask, words, seqs, max_q_len, heads, kv_heads, head_dim, scale, int(window or 0), splits, status, _stream())
+        _refuse_maps(rc, "attention's")
+        _check(rc, "attention_tree")
+        return out
+    if kernel == "mma":
+        row_warps, splits = _tree_mma_plan(max_q_len * group, kv_heads * seqs, keys)
+        if parts is not None:
+            row_warps, splits = parts
+        acc = ml = None
+        if splits > 8:
+            acc = _empty(q, (q.shape[0] * heads * splits * head_dim,), torch.float32)
+            ml = _empty(q, (q.shape[0] * heads * splits * 2,), torch.float32)
+        rc = _lib("attention_tree_mma").sb_attention_tree_mma(
+            q, out, k_store, v_store, block_table, block_table.shape[1], seq_slot, seq_q_start, seq_q_len, seq_kv_len, tok_pos, tree_mask,
+            words, seqs, max_q_len, heads, kv_heads, head_dim, scale, int(window or 0), splits, row_warps, acc, ml, _stream())
+        _check(rc, "attention_tree", 2 if splits > 8 else 1)
+        return out
+    splits = _tree_plain_splits(-(-max_q_len * group // 16) * kv_heads * seqs, keys)
     acc = ml = None
     if splits > 1:
         acc = _empty(q, (q.shape[0] * heads * splits * head_dim,), torch.float32)

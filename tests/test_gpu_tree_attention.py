@@ -271,6 +271,37 @@ def test_captured_on_another_stream_and_replayed(dtype, dim, nodes):
         check(c, out)
 
 
+@pytest.mark.parametrize("dim, group, nodes", [(128, 4, 64), (64, 8, 20), (128, 3, 100), (128, 1, 256), (64, 7, 40), (128, 16, 9)])
+@pytest.mark.parametrize("parts", [1, 2, 4, 8])
+def test_keys_in_parts_on_tensor_memory(dim, group, nodes, parts):
+    sees, depth = trees([nodes, 1, nodes // 2], seed=nodes)
+    for past, window in (([700, 64, 0], None), ([1500, 300, 1023], 200)):
+        c = Case("bf16", 2 * group, 2, dim, sees, past, depth, window=window, seed=nodes)
+        check(c, ops.attention_tree(**c.on_device(), kernel="tcgen05", parts=parts))
+
+
+@pytest.mark.parametrize("dim", [16, 32, 64, 128])
+@pytest.mark.parametrize("parts", [(1, 1), (1, 5), (2, 3), (2, 8), (4, 2), (4, 7), (1, 9), (2, 17), (4, 32)])
+def test_keys_in_parts_on_warps(dim, parts):
+    sees, depth = trees([21, 1, 0, 40], seed=dim)
+    c = Case("bf16", 6, 2, dim, sees, [800, 64, 0, 129], depth, window=300 if parts[1] % 2 else None, seed=dim)
+    check(c, ops.attention_tree(**c.on_device(), kernel="mma", parts=parts))
+
+
+@pytest.mark.parametrize("parts", [1, 2])
+def test_a_wait_of_the_tree_attention_that_runs_out_is_reported(parts):
+    """Half of a step's values are not copied: the wait gives up, the status says so, and the next call is right."""
+    sees, depth = trees([64], seed=2)
+    c = Case("bf16", 8, 2, 128, sees, [500], depth, seed=2)
+    status = torch.zeros((1,), dtype=torch.int32, device="cuda")
+    ops.attention_tree(**c.on_device(), kernel="tcgen05", parts=parts, status=status, withhold=(1, 2_000_000))
+    torch.cuda.synchronize()
+    assert status.item() == 16
+    status.zero_()
+    check(c, ops.attention_tree(**c.on_device(), kernel="tcgen05", parts=parts, status=status))
+    assert status.item() == 0
+
+
 def test_refusals():
     sees, depth = trees([5])
     c = Case("bf16", 4, 2, 64, sees, [10], depth)
