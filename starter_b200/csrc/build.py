@@ -71,6 +71,7 @@ SOURCES = (
     "attention_tree_tc",
     "cache_pages",
     "token_logprobs",
+    "score_tcgen05",
 )
 
 _lock = threading.Lock()

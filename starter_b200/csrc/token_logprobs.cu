@@ -9,29 +9,13 @@
 // are no numbers are never listed.
 //
 // A row is shared by the blocks of a cluster, whose results meet in the first one's hands.  What bounds it is reading the logits.
-#include "common.cuh"
+#include "logprob_stats.cuh"
 
 #define LP_THREADS 256
 #define LP_WARPS (LP_THREADS / 32)
 #define LP_MAX_TOP 32
 #define LP_MAX_CLUSTER 8
 #define LP_NONE 0x7fffffff
-
-struct Stats { float m, l, t; };
-
-__device__ __forceinline__ float lp_exp(float d) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(d * 1.4426950408889634f));
-  return y;
-}
-// Both parts on the larger reference.  (A part that has seen no finite entry has m = -inf, L = T = 0.)
-__device__ __forceinline__ Stats lp_join(const Stats& a, const Stats& b) {
-  const float m = fmaxf(a.m, b.m), base = m == -INFINITY ? 0.f : m;
-  const float da = fmaxf(a.m - base, -1e30f), db = fmaxf(b.m - base, -1e30f);
-  const float wa = lp_exp(da), wb = lp_exp(db);
-  // (a weight of zero meets a distance of 1e30 here: L is then 0 or its part is)
-  return Stats{m, fmaf(a.l, wa, b.l * wb), wa * fmaf(a.l, wa > 0.f ? da : 0.f, a.t) + wb * fmaf(b.l, wb > 0.f ? db : 0.f, b.t)};
-}
 
 struct Item { float v; int i; };
 __device__ __forceinline__ bool lp_before(const Item& a, const Item& b) { return a.v > b.v || (a.v == b.v && a.i < b.i); }

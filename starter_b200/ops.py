@@ -1280,11 +1280,13 @@ def _refuse_rows(t, name):
 LOGPROBS_CHUNK_BYTES = 256 << 20
 
 
-def linear_logprobs(h, weight, tokens, softcap=None, status=None):
+def linear_logprobs(h, weight, tokens, softcap=None, status=None, withhold=None):
     """``token_logprobs`` of ``h @ weight.T`` without alternatives: ``(logprob, entropy)``, float32 ``[R]`` each.
 
     ``h`` ``[R, K]`` are hidden rows behind the final norm, ``weight`` ``[V, K]`` the head, of the same type; ``softcap`` (None: none)
-    caps the logits as ``ops.softcap`` does."""
+    caps the logits as ``ops.softcap`` does.  In bfloat16 with more than 128 rows the logits are never in memory (csrc/score_tcgen05.cu);
+    otherwise they are formed ``LOGPROBS_CHUNK_BYTES`` at a time.  ``withhold = (k_block, limit_ns)`` is for tests of the kernel's give-up
+    path: one copy is left out, a wait runs out after ``limit_ns``, bit 4 of ``status`` is set and the result is undefined."""
     _need(h, "h", None, 2)
     _need(weight, "weight", h.dtype, 2)
     _need(tokens, "tokens", torch.int32, 1)
@@ -1297,6 +1299,17 @@ def linear_logprobs(h, weight, tokens, softcap=None, status=None):
     if vocab == 0 or h.shape[1] == 0:
         raise KernelError(f"a head of shape {tuple(weight.shape)} gives no logits")
     out = _empty(h, (2, rows), torch.float32)
+    if softcap is not None and not softcap > 0:
+        raise KernelError(f"a cap of {softcap}")
+    if h.dtype == torch.bfloat16 and rows > TENSOR_CORE_MAX_ROWS and h.shape[1] % 8 == 0 and not (h.data_ptr() | weight.data_ptr()) & 15:
+        lib = _lib("score_tcgen05")
+        if withhold is not None:
+            lib.sb_score_withhold(int(withhold[0]), int(withhold[1]))
+        scratch = _empty(h, (lib.sb_score_scratch(rows, vocab),), torch.float32)
+        rc = lib.sb_score(h, weight, tokens, rows, vocab, h.shape[1], float(softcap or 0.0), out[0], out[1], scratch, status, _stream())
+        _refuse_maps(rc, "score's")
+        _check(rc, "linear_logprobs", 2)
+        return out[0], out[1]
     chunk = max(1, LOGPROBS_CHUNK_BYTES // (4 * vocab))
     for first in range(0, rows, chunk):
         logits = linear(h[first:first + chunk], weight, out_float=True, status=status)

@@ -264,6 +264,18 @@ def test_score_captured_and_replayed():
     assert torch.equal(out[0], again[0]) and torch.equal(out[1], again[1])
 
 
+def test_a_wait_of_the_score_that_runs_out_is_reported():
+    h, w, t = score_case(300, 256, 3000, torch.bfloat16, 5)
+    status = torch.zeros((1,), dtype=torch.int32, device="cuda")
+    ops.linear_logprobs(h, w, t, status=status, withhold=(1, 2_000_000))
+    torch.cuda.synchronize()
+    assert status.item() == 4
+    status.zero_()
+    ops.linear_logprobs(h, w, t, status=status)
+    check_score(h, w, t)
+    assert status.item() == 0
+
+
 def test_score_refusals():
     h, w, t = score_case(5, 64, 900, torch.bfloat16, 2)
     for args in ((h.float(), w, t), (h, w[:, :32].contiguous(), t), (h, w, t[:-1]), (h, w, t.long()), (h[0], w, t), (h, w[:0], t), (h.half(), w.half(), t),
