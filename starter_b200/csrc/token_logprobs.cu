@@ -3,10 +3,15 @@
 // With m a row's largest entry, L = sum exp(x_i - m) and T = sum exp(x_i - m) (x_i - m):
 //     lse = m + log L,   log p(t) = (x_t - m) - log L,   H = log L - T / L.
 // Every thread keeps (m, L, T) of what it has seen, all float; a new reference m' scales L by a = exp(m - m') and makes
-// T a (T + L (m - m')).  Entries of minus infinity add nothing to any of them.  The alternatives are the largest entries, the lowest
-// index first among equals: a warp keeps the best 32 it has seen, sorted, one to a lane, and looks closer only at tiles whose largest
-// entry beats its k-th (or is not worse than the best k-th any warp of the block has: k entries above it are known then).  Entries that
-// are no numbers are never listed.
+// T a (T + L (m - m')).  Entries of minus infinity add nothing to any of them.
+//
+// The alternatives are the k largest entries, the lowest index first among equals.  The pass itself leaves only the largest entry of every 64
+// bytes of the row in shared memory: of such groups, ordered by their largest entry and then by place, the first k hold all alternatives
+// (an entry of another group has k entries in front of it).  Behind the pass the block finds those groups and reads them once more: a bar that k + 1
+// of them reach comes from the threads' best ones, what reaches it is ranked by counting, and so are the groups' entries.  A value and
+// an index make one 64-bit key, larger for what comes first, so that all keys differ.  (Candidates gathered in the pass itself, into a sorted
+// list a warp or a buffer a block, cost barriers and divergent code in every tile: 8 rows of 151,936 with 20 alternatives 30 and 17 us, 600
+// rows with 5 110 and 138.)  Entries that are no numbers have no key.
 //
 // A row is shared by the blocks of a cluster, whose results meet in the first one's hands.  What bounds it is reading the logits.
 #include "logprob_stats.cuh"
@@ -15,24 +20,21 @@
 #define LP_WARPS (LP_THREADS / 32)
 #define LP_MAX_TOP 32
 #define LP_MAX_CLUSTER 8
-#define LP_NONE 0x7fffffff
+#define LP_BYTES 64                      // a thread's piece of a tile: a group
+#define LP_TILE_BYTES (LP_THREADS * LP_BYTES)
+#define LP_QUADS (LP_THREADS / 4)
+#define LP_BUFFER 1088                   // keys: the entries of LP_MAX_TOP + 1 groups, and a cluster's lists
+#define LP_MAX_SLOTS 160                 // tiles of a block whose groups' largest entries shared memory holds
 
-struct Item { float v; int i; };
-__device__ __forceinline__ bool lp_before(const Item& a, const Item& b) { return a.v > b.v || (a.v == b.v && a.i < b.i); }
-__device__ __forceinline__ Item lp_shfl(const Item& a, int lane) {
-  return Item{__shfl_sync(0xffffffffu, a.v, lane), __shfl_sync(0xffffffffu, a.i, lane)};
+typedef unsigned long long Key;
+// 0: none.  (Both zeros are one value.)
+__device__ __forceinline__ Key lp_key(float v, int i) {
+  const uint32_t b = __float_as_uint(v + 0.f);
+  return v == v ? (Key)(b & 0x80000000u ? ~b : b | 0x80000000u) << 32 | (uint32_t)~i : 0ull;
 }
-// The best 32 of two sorted lists (best in lane 0): the other one backwards against this one leaves them as a bitonic sequence.
-__device__ __forceinline__ Item lp_merge(Item a, const Item& b_lane) {
-  const int lane = threadIdx.x & 31;
-  const Item b = lp_shfl(b_lane, 31 - lane);
-  if (lp_before(b, a)) a = b;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const Item other{__shfl_xor_sync(0xffffffffu, a.v, o), __shfl_xor_sync(0xffffffffu, a.i, o)};
-    if (lp_before(other, a) == ((lane & o) == 0)) a = other;
-  }
-  return a;
+__device__ __forceinline__ float lp_value(Key k) {
+  const uint32_t b = (uint32_t)(k >> 32);
+  return __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~b);
 }
 
 struct LogprobArgs {
@@ -57,74 +59,88 @@ __device__ __forceinline__ float lp_peer_load(uint32_t a) {
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
   return v;
 }
-
+__device__ __forceinline__ Key lp_peer_key(uint32_t a) {
+  Key v;
+  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
+  return v;
+}
 __device__ __forceinline__ void lp_cluster_barrier() {
   __syncwarp();                    // (.aligned: a whole warp at once)
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// 32 bytes on their boundary, which are not needed again.
+__device__ __forceinline__ void lp_load32(uint32_t* w, const void* p) {
+  asm volatile("ld.global.cs.v4.b64 {%0, %1, %2, %3}, [%4];"
+               : "=l"(reinterpret_cast<Key*>(w)[0]), "=l"(reinterpret_cast<Key*>(w)[1]), "=l"(reinterpret_cast<Key*>(w)[2]), "=l"(reinterpret_cast<Key*>(w)[3])
+               : "l"(p));
+}
+
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(LP_THREADS) token_logprobs_kernel(const LogprobArgs a, int parts) {
-  constexpr int VEC = 16 / sizeof(T), U = 16 / VEC;       // entries of a 16-byte load; loads a thread has on their way
-  constexpr int N = VEC * U;
+__global__ void __launch_bounds__(LP_THREADS, 4) token_logprobs_kernel(const LogprobArgs a, int rest) {
+  constexpr int N = LP_BYTES / sizeof(T), HALF = N / 2;   // entries of a thread's piece, in two loads
+  extern __shared__ float maxima[];                       // [tiles of this block][LP_THREADS]
   __shared__ float sh_stats[LP_WARPS][3], cl_stats[3];
-  __shared__ float sh_v[LP_WARPS][32], cl_v[32];
-  __shared__ int sh_i[LP_WARPS][32], cl_i[32];
-  __shared__ float sh_floor;                              // the best k-th entry any warp has
+  __shared__ Key buffer[TOP ? LP_BUFFER : 1], list[LP_MAX_TOP + 1], quad_best[LP_QUADS], sh_bar;
+  __shared__ int sh_count;
+  // A launch whose rows are the rest of the one directly in front of it (`rest`) reads the logits while that one still runs: its blocks are there
+  // once every block of the other has passed its own wait, which the logits were complete for.  It waits in front of its first write.
+  if (!rest) pdl_wait();
   pdl_trigger();
-  pdl_wait();
-  const int row = blockIdx.y, part = blockIdx.x;
+  const int row = blockIdx.y, parts = gridDim.x, part = blockIdx.x;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const T* x = (const T*)a.logits + (size_t)row * a.row_stride;
-  // loads start on 16-byte boundaries: the row is `off` entries behind one
-  const int off = (int)(((uintptr_t)x & 15) / sizeof(T));
-  const T* aligned = x - off;
-  if (threadIdx.x == 0) sh_floor = -INFINITY;
-  __syncthreads();
-
-  const long long vectors = ((long long)off + a.vocab + VEC - 1) / VEC;
-  const int per_tile = LP_THREADS * U;
-  const int tiles = (int)((vectors + per_tile - 1) / per_tile);
-  Stats st{-INFINITY, 0.f, 0.f};
-  Item best{-INFINITY, LP_NONE}, kth{-INFINITY, LP_NONE};
-  uint4 raw[U];
-  auto load = [&](int tile) {
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const long long first = ((long long)tile * per_tile + u * LP_THREADS + threadIdx.x) * VEC - off;    // of the row
-      if (first >= 0 && first + VEC <= a.vocab) {
-        raw[u] = __ldcs(reinterpret_cast<const uint4*>(x + first));
-      } else {                                            // the row's ends, entry by entry; minus infinity beside them
-        T e[VEC];
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) e[i] = first + i >= 0 && first + i < a.vocab ? x[first + i] : from_f<T>(-INFINITY);
-        raw[u] = *reinterpret_cast<uint4*>(e);
-      }
-    }
+  // loads start on 32-byte boundaries: the row is `off` entries behind one
+  const int off = (int)(((uintptr_t)x & 31) / sizeof(T));
+  const int tiles = (int)(((long long)off + a.vocab + LP_THREADS * N - 1) / (LP_THREADS * N));
+  const int slots = part < tiles ? (tiles - part + parts - 1) / parts : 0;
+  auto first_of = [&](int slot, int thread) -> long long {   // the first entry of a thread's piece of a tile
+    return ((long long)(part + slot * parts) * LP_THREADS + thread) * N - off;
   };
-  if (part < tiles) load(part);
-  for (int tile = part; tile < tiles; tile += parts) {
-    float v[N];
+  Stats st{-INFINITY, 0.f, 0.f};
+  int best_slot = -1;                                     // the tile of the thread's largest entry
+  uint32_t raw[LP_BYTES / 4];
+  auto load = [&](int slot) {
+    const long long first = first_of(slot, threadIdx.x);
+    if (first >= 0 && first + N <= a.vocab) {
+      lp_load32(raw, x + first);
+      lp_load32(raw + LP_BYTES / 8, x + first + HALF);
+    } else {                                              // the row's ends, entry by entry; minus infinity beside them
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int w = 0; w < LP_BYTES / 4; ++w) {
         if constexpr (sizeof(T) == 4) {
-          v[u * VEC + i] = __uint_as_float(w[i]);
+          raw[w] = first + w >= 0 && first + w < a.vocab ? reinterpret_cast<const uint32_t*>(x)[first + w] : 0xff800000u;
         } else {
-          v[u * VEC + 2 * i] = __uint_as_float(w[i] << 16);
-          v[u * VEC + 2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+          const long long e = first + 2 * w;
+          const uint32_t lo = e >= 0 && e < a.vocab ? reinterpret_cast<const uint16_t*>(x)[e] : 0xff80u;
+          const uint32_t hi = e + 1 >= 0 && e + 1 < a.vocab ? reinterpret_cast<const uint16_t*>(x)[e + 1] : 0xff80u;
+          raw[w] = lo | hi << 16;
         }
       }
     }
-    if (tile + parts < tiles) load(tile + parts);
+  };
+  int slot = slots ? row * 11 % slots : 0;
+  if (slots) load(slot);
+  for (int n = 0; n < slots; ++n) {
+    const int next = slot + 1 < slots ? slot + 1 : 0;
+    float v[N];
+#pragma unroll
+    for (int w = 0; w < LP_BYTES / 4; ++w) {
+      if constexpr (sizeof(T) == 4) {
+        v[w] = __uint_as_float(raw[w]);
+      } else {
+        v[2 * w] = __uint_as_float(raw[w] << 16);
+        v[2 * w + 1] = __uint_as_float(raw[w] & 0xffff0000u);
+      }
+    }
+    if (n + 1 < slots) load(next);
     float mx = v[0];
 #pragma unroll
     for (int e = 1; e < N; ++e) mx = fmaxf(mx, v[e]);
+    if (TOP) maxima[slot * LP_THREADS + threadIdx.x] = mx;
     if (mx > st.m) {
-      const Stats here{mx, 0.f, 0.f};
-      st = lp_join(st, here);
+      st = lp_join(st, Stats{mx, 0.f, 0.f});
+      best_slot = slot;
     }
     const float base = st.m == -INFINITY ? 0.f : st.m;
 #pragma unroll
@@ -133,28 +149,94 @@ __global__ void __launch_bounds__(LP_THREADS) token_logprobs_kernel(const Logpro
       st.l += p;
       st.t = fmaf(p, fmaxf(d, -1e30f), st.t);
     }
-    if constexpr (TOP) {
-      const float floor = *(volatile float*)&sh_floor;
-      if (__any_sync(0xffffffffu, (mx > kth.v || kth.i == LP_NONE) && mx >= floor)) {
+    slot = next;
+  }
+
+  // The `want` best of the buffer's `count` keys to list, in order (zeros behind them).  Every thread, between barriers.
+  auto rank = [&](int count, int want) {
+    if (threadIdx.x <= LP_MAX_TOP) list[threadIdx.x] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < count; i += LP_THREADS) {
+      const Key mine = buffer[i];
+      int above = 0;
+      for (int j = 0; j < count; ++j) above += buffer[j] > mine;
+      if (above < want) list[above] = mine;
+    }
+    __syncthreads();
+  };
+  if constexpr (TOP) {
+    // One group more than alternatives: the row's first one may begin in front of the row, and name what stands there its best.
+    const int want = a.top + 1;
+    auto group_key = [&](int slot) { return lp_key(maxima[slot * LP_THREADS + threadIdx.x], slot * LP_THREADS + threadIdx.x); };
+    Key best = 0;
+    if (best_slot >= 0) best = lp_key(st.m, best_slot * LP_THREADS + threadIdx.x);
+    else                                                  // (nothing above minus infinity)
+      for (int s = 0; s < slots; ++s) best = max(best, group_key(s));
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-          const long long place = ((long long)tile * per_tile + (e / VEC) * LP_THREADS + threadIdx.x) * VEC + e % VEC - off;
-          const Item mine{v[e], place >= 0 && place < a.vocab ? (int)place : LP_NONE};
-          uint32_t left = __ballot_sync(0xffffffffu, lp_before(mine, kth) && mine.v >= floor);
-          while (left) {
-            const Item cand = lp_shfl(mine, __ffs(left) - 1);
-            left &= left - 1;
-            if (!lp_before(cand, kth)) continue;          // (the same in every lane)
-            const int at = __popc(__ballot_sync(0xffffffffu, lp_before(best, cand)));
-            const Item up{__shfl_up_sync(0xffffffffu, best.v, 1), __shfl_up_sync(0xffffffffu, best.i, 1)};
-            if (lane == at) best = cand;
-            else if (lane > at) best = up;
-            kth = lp_shfl(best, a.top - 1);
-          }
+    for (int o = 1; o < 4; o <<= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+    if ((lane & 3) == 0) quad_best[threadIdx.x / 4] = best;
+    if (threadIdx.x == 0) sh_count = 0;
+    __syncthreads();
+    if (threadIdx.x < LP_QUADS) {
+      const Key mine = quad_best[threadIdx.x];
+      int above = 0;
+#pragma unroll 8
+      for (int j = 0; j < LP_QUADS; ++j) above += quad_best[j] > mine || (quad_best[j] == mine && j < threadIdx.x);
+      if (above == want - 1) sh_bar = mine;               // `want` groups reach it (or there are not that many, and it is 0)
+    }
+    __syncthreads();
+    {
+      const Key bar = sh_bar;
+      const float value = bar ? lp_value(bar) : -INFINITY;
+#pragma unroll 8
+      for (int s = 0; s < slots; ++s) {
+        if (!(maxima[s * LP_THREADS + threadIdx.x] >= value)) continue;
+        const Key key = group_key(s);
+        if (key >= bar) {
+          const int at = atomicAdd(&sh_count, 1);
+          if (at < LP_BUFFER) buffer[at] = key;
         }
-        if (lane == 0 && kth.i != LP_NONE && kth.v > floor) *(volatile float*)&sh_floor = kth.v;   // (any warp's is true; a lost race costs a look)
       }
     }
+    __syncthreads();
+    int count = sh_count;
+    if (count <= LP_BUFFER) {
+      rank(count, want);
+    } else {
+      // (a few threads hold far more of the best groups than their share: the best of all, the best below it, and so on)
+      Key last = ~0ull;
+      for (int n = 0; n < want; ++n) {
+        Key mine = 0;
+        for (int s = 0; s < slots; ++s) {
+          const Key key = group_key(s);
+          if (key < last) mine = max(mine, key);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, o));
+        if (lane == 0) quad_best[warp] = mine;
+        __syncthreads();
+        last = 0;
+        for (int w = 0; w < LP_WARPS; ++w) last = max(last, quad_best[w]);
+        if (threadIdx.x == 0) list[n] = last;
+        __syncthreads();
+      }
+    }
+    // the groups' entries that reach the k-th group's best
+    const float bar = list[a.top - 1] ? lp_value(list[a.top - 1]) : -INFINITY;
+    if (threadIdx.x == 0) sh_count = 0;
+    __syncthreads();
+    for (int idx = threadIdx.x; idx < want * N; idx += LP_THREADS) {
+      const Key group = list[idx / N];
+      if (group == 0) break;
+      const int id = (int)~(uint32_t)group;
+      const long long place = first_of(id / LP_THREADS, id % LP_THREADS) + idx % N;
+      if (place < 0 || place >= a.vocab) continue;
+      const float value = to_f<T>(x[place]);
+      if (value >= bar) buffer[atomicAdd(&sh_count, 1)] = lp_key(value, (int)place);
+    }
+    __syncthreads();
+    count = sh_count;
+    rank(count, a.top);
   }
 
   // the lanes', then the warps', then the blocks' parts
@@ -164,19 +246,7 @@ __global__ void __launch_bounds__(LP_THREADS) token_logprobs_kernel(const Logpro
     st = lp_join(st, other);
   }
   if (lane == 0) { sh_stats[warp][0] = st.m; sh_stats[warp][1] = st.l; sh_stats[warp][2] = st.t; }
-  if (TOP) { sh_v[warp][lane] = best.v; sh_i[warp][lane] = best.i; }
   __syncthreads();
-  auto fold = [&]() {                                     // the lists of sh_v, sh_i into warp 0's registers
-    for (int half = LP_WARPS / 2; half > 0; half >>= 1) {
-      if (warp < half) {
-        best = lp_merge(best, Item{sh_v[warp + half][lane], sh_i[warp + half][lane]});
-        sh_v[warp][lane] = best.v;
-        sh_i[warp][lane] = best.i;
-      }
-      __syncthreads();
-    }
-  };
-  if (TOP) fold();
   if (warp == 0) {
     st = lane < LP_WARPS ? Stats{sh_stats[lane][0], sh_stats[lane][1], sh_stats[lane][2]} : Stats{-INFINITY, 0.f, 0.f};
 #pragma unroll
@@ -188,21 +258,13 @@ __global__ void __launch_bounds__(LP_THREADS) token_logprobs_kernel(const Logpro
   if (parts > 1) {
     if (warp == 0) {
       if (lane == 0) { cl_stats[0] = st.m; cl_stats[1] = st.l; cl_stats[2] = st.t; }
-      if (TOP) { cl_v[lane] = best.v; cl_i[lane] = best.i; }
     }
     __syncthreads();
     lp_cluster_barrier();
     if (part == 0) {
       if (TOP) {
-        best = Item{-INFINITY, LP_NONE};
-        if (warp < parts) {
-          best.v = lp_peer_load(lp_peer(&cl_v[lane], warp));
-          best.i = __float_as_int(lp_peer_load(lp_peer(&cl_i[lane], warp)));
-        }
-        sh_v[warp][lane] = best.v;
-        sh_i[warp][lane] = best.i;
+        for (int i = threadIdx.x; i < parts * a.top; i += LP_THREADS) buffer[i] = lp_peer_key(lp_peer(&list[i % a.top], i / a.top));
         __syncthreads();
-        fold();
       }
       if (warp == 0) {
         st = Stats{-INFINITY, 0.f, 0.f};
@@ -217,8 +279,10 @@ __global__ void __launch_bounds__(LP_THREADS) token_logprobs_kernel(const Logpro
     }
     lp_cluster_barrier();                                 // nobody leaves while it is read
     if (part) return;
+    if (TOP) rank(parts * a.top, a.top);
   }
   if (warp == 0) {
+    if (rest) pdl_wait();
     // (a sum that is no number, or of nothing, makes a row whose probabilities are none)
     const float log_l = st.l > 0.f ? logf(st.l) : NAN;
     if (lane == 0) {
@@ -234,42 +298,73 @@ __global__ void __launch_bounds__(LP_THREADS) token_logprobs_kernel(const Logpro
       a.entropy[row] = log_l - st.t / st.l;
     }
     if (TOP && lane < a.top) {
-      a.top_value[(size_t)row * a.top + lane] = (best.v - st.m) - log_l;
-      a.top_id[(size_t)row * a.top + lane] = best.i == LP_NONE ? -1 : best.i;
+      const Key key = list[lane];
+      a.top_value[(size_t)row * a.top + lane] = ((key ? lp_value(key) : -INFINITY) - st.m) - log_l;
+      a.top_id[(size_t)row * a.top + lane] = key ? (int)~(uint32_t)key : -1;
     }
   }
 }
 
+// Tiles of a block with the most of them.
+template <typename T> static int lp_slots(int vocab, int parts) {
+  const long long tiles = ((long long)vocab + 31 / (int)sizeof(T) + LP_TILE_BYTES / (int)sizeof(T) - 1) / (LP_TILE_BYTES / (int)sizeof(T));
+  return (int)((tiles + parts - 1) / parts);
+}
+
 template <typename T, bool TOP>
-static int launch_rows(const LogprobArgs& a, int rows, int parts, cudaStream_t s) {
-  for (int first = 0; first < rows; first += 65535) {     // (a grid's dimension)
-    LogprobArgs b = a;
-    const int here = rows - first < 65535 ? rows - first : 65535;
-    b.logits = (const T*)a.logits + (size_t)first * a.row_stride;
-    b.tokens += first; b.given += first; b.entropy += first;
-    if (TOP) { b.top_value += (size_t)first * a.top; b.top_id += (size_t)first * a.top; }
-    const int rc = launch_dependent_cluster(token_logprobs_kernel<T, TOP>, dim3(parts, here), dim3(LP_THREADS), 0, s, dim3(parts), b, parts);
+static int launch_rows(LogprobArgs a, int first, int rows, int parts, int rest, cudaStream_t s) {
+  int smem = 0;
+  if (TOP) {
+    // (with less than the launch in front of it, an SM would have to be empty before it could divide its memory anew)
+    const int slots = lp_slots<T>(a.vocab, rest ? 1 : parts);
+    if (slots > LP_MAX_SLOTS) return -2;
+    smem = slots * LP_THREADS * 4;
+    // (an attribute of the device the launch goes to)
+    const cudaError_t e = cudaFuncSetAttribute(token_logprobs_kernel<T, TOP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return (int)e;
+  }
+  a.logits = (const T*)a.logits + (size_t)first * a.row_stride;
+  a.tokens += first; a.given += first; a.entropy += first;
+  if (TOP) { a.top_value += (size_t)first * a.top; a.top_id += (size_t)first * a.top; }
+  while (rows > 0) {                                      // (a grid's dimension counts 65,535 rows)
+    const int here = rows < 65535 ? rows : 65535;
+    const int rc = launch_dependent_cluster(token_logprobs_kernel<T, TOP>, dim3(parts, here), dim3(LP_THREADS), smem, s, dim3(parts), a, rest);
     if (rc) return rc;
+    a.logits = (const T*)a.logits + (size_t)here * a.row_stride;
+    a.tokens += here; a.given += here; a.entropy += here;
+    if (TOP) { a.top_value += (size_t)here * a.top; a.top_id += (size_t)here * a.top; }
+    rows -= here;
+    rest = 0;
   }
   return 0;
+}
+template <typename T, bool TOP>
+static int launch_all(const LogprobArgs& a, int rows, int whole, int parts, cudaStream_t s) {
+  const int rc = whole ? launch_rows<T, TOP>(a, 0, whole, 1, 0, s) : 0;
+  return rc || whole == rows ? rc : launch_rows<T, TOP>(a, whole, rows - whole, parts, whole > 0, s);
 }
 
 extern "C" {
 
-int sb_token_logprobs_max_top() { return LP_MAX_TOP; }
+// The longest rows whose alternatives can be listed: LP_MAX_SLOTS tiles in each of a cluster's blocks.
+long long sb_token_logprobs_max_vocab(int dtype) {
+  return (long long)LP_MAX_CLUSTER * LP_MAX_SLOTS * (LP_TILE_BYTES / (dtype == 0 ? 4 : 2)) - 32;
+}
 
 // logits: [rows, vocab], dtype 0 float, 1 bfloat16, rows `row_stride` entries apart; tokens [rows]; top 0 to 32, at most vocab;
-// given, entropy [rows]; top_value, top_id [rows, top] (null with top 0); parts: 1, 2, 4 or 8 blocks a row.  A token of vocab or more sets
-// bit 1 of *status (null: not told) and has no log probability.
+// given, entropy [rows]; top_value, top_id [rows, top] (null with top 0).  The first `whole` rows have a block each,
+// the others `parts` blocks (1, 2, 4 or 8); with alternatives a block takes at most 160 tiles of 16 KB.  A token of vocab or more sets bit
+// 1 of *status (null: not told) and has no log probability.
 int sb_token_logprobs(int dtype, const void* logits, int rows, int vocab, long long row_stride, const int* tokens, int top, float* given,
-                      float* entropy, float* top_value, int* top_id, int parts, int* status, cudaStream_t s) {
+                      float* entropy, float* top_value, int* top_id, int whole, int parts, int* status, cudaStream_t s) {
   if (rows == 0) return 0;
   if (vocab < 1 || top < 0 || top > LP_MAX_TOP || top > vocab || row_stride < 0) return -2;
   if (parts != 1 && parts != 2 && parts != 4 && parts != LP_MAX_CLUSTER) return -2;
-  if (vocab > 0x7fffff00 || ((uintptr_t)logits & (dtype == 0 ? 3 : 1))) return -2;
+  if (whole < 0 || whole > rows) return -2;
+  if (vocab > 0x7fff0000 || ((uintptr_t)logits & (dtype == 0 ? 3 : 1))) return -2;
   const LogprobArgs a{logits, row_stride, vocab, top, tokens, given, entropy, top_value, top_id, status};
-  if (dtype == 0) return top ? launch_rows<float, true>(a, rows, parts, s) : launch_rows<float, false>(a, rows, parts, s);
-  if (dtype == 1) return top ? launch_rows<bf16, true>(a, rows, parts, s) : launch_rows<bf16, false>(a, rows, parts, s);
+  if (dtype == 0) return top ? launch_all<float, true>(a, rows, whole, parts, s) : launch_all<float, false>(a, rows, whole, parts, s);
+  if (dtype == 1) return top ? launch_all<bf16, true>(a, rows, whole, parts, s) : launch_all<bf16, false>(a, rows, whole, parts, s);
   return -1;
 }
 

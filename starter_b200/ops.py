@@ -1229,12 +1229,25 @@ def _here(t, name):
 LOGPROBS_MAX_TOP = 32
 
 
-def _logprob_parts(rows: int, vocab: int) -> int:
-    """How many blocks (a cluster) share a row of logits: as many as keep two blocks on every SM."""
-    parts = 1
-    while parts < 8 and 2 * parts * rows <= 2 * SM_COUNT and 2 * parts * 4096 <= vocab:
+#: the longest rows of float32 logits whose alternatives ``token_logprobs`` lists (twice as long in bfloat16)
+LOGPROBS_MAX_VOCAB = 8 * 160 * 4096 - 32
+
+
+@functools.lru_cache(maxsize=4096)
+def _logprob_plan(rows: int, row_bytes: int) -> tuple:
+    """``(whole, parts)``: how many rows of logits have a block of their own, and how many blocks (a cluster) share each of the others.
+
+    Four blocks run on an SM.  Full waves of them take whole rows; what is left over is cut so that it fills the SMs once more, down to
+    two of a block's tiles of 16 KB, and runs into the last wave's end."""
+    places, tiles = 4 * SM_COUNT, -(-row_bytes // 16384)
+    left, parts = rows % places, 1
+    while parts < 8 and 2 * parts * left <= places and 4 * parts <= tiles:
         parts *= 2
-    return parts
+    if tiles > 160:                          # (more than a block's shared memory holds the groups of)
+        while -(-tiles // parts) > 160:
+            parts *= 2
+        return 0, parts
+    return (rows if left == 0 or parts == 1 else rows - left), parts
 
 
 def token_logprobs(logits, tokens, top=0, status=None):
@@ -1255,13 +1268,16 @@ def token_logprobs(logits, tokens, top=0, status=None):
         raise KernelError(f"{tokens.shape[0]} tokens for {rows} rows of logits")
     if not 0 <= top <= min(LOGPROBS_MAX_TOP, vocab):
         raise KernelError(f"{top} alternatives asked for; the kernel lists 0 to {min(LOGPROBS_MAX_TOP, vocab)} of {vocab}")
+    if top and vocab * logits.element_size() > 4 * LOGPROBS_MAX_VOCAB:
+        raise KernelError(f"alternatives of rows of {vocab} entries; {4 * LOGPROBS_MAX_VOCAB // logits.element_size()} are the most")
     out = _empty(tokens, (2, rows), torch.float32)
     values, ids = _empty(tokens, (rows, top), torch.float32), _empty(tokens, (rows, top), torch.int32)
     if rows:
+        whole, parts = _logprob_plan(rows, vocab * logits.element_size())
         rc = _lib("token_logprobs").sb_token_logprobs(
-            _code(logits.dtype), logits, rows, vocab, logits.stride(0), tokens, top, out[0], out[1], values, ids,
-            _logprob_parts(rows, vocab), status, _stream())
-        _check(rc, "token_logprobs", -(-rows // 65535))
+            _code(logits.dtype), logits, rows, vocab, logits.stride(0), tokens, top, out[0], out[1], values, ids, whole, parts, status,
+            _stream())
+        _check(rc, "token_logprobs", 2 if 0 < whole < rows else 1)
     return out[0], out[1], values, ids
 
 

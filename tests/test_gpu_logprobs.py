@@ -69,7 +69,7 @@ def test_sizes_of_vocabularies(dtype, vocab):
                 check(x, t, top)
 
 
-@pytest.mark.parametrize("rows", [1, 2, 18, 19, 37, 38, 74, 75, 148, 149, 700])
+@pytest.mark.parametrize("rows", [1, 2, 18, 19, 37, 38, 74, 75, 148, 149, 296, 297, 592, 593, 600, 666, 700, 889, 1184, 1186])
 def test_numbers_of_rows(rows):
     x, t = logits(rows, 33333, rows)
     check(x, t, 20)
@@ -155,6 +155,28 @@ def test_tokens_that_are_none():
 def test_more_rows_than_a_grid_dimension_counts():
     x, t = logits(66000, 40, 9)
     check(x, t, 3)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_alternatives_of_very_long_rows(dtype):
+    for vocab in (700_001, 2_000_003, 5_242_000):
+        x, t = logits(2, vocab, vocab, dtype)
+        _, _, values, ids = ops.token_logprobs(x, t, top=32)
+        order = torch.sort(x, dim=1, descending=True, stable=True).indices[:, :32]
+        assert torch.equal(ids, order.int())
+    with pytest.raises(KernelError):
+        ops.token_logprobs(logits(1, 11_000_000, 1, dtype)[0], t[:1], top=1)
+
+
+def test_groups_that_hold_more_than_their_share():
+    """The best entries in a few threads' pieces of every tile, and in ascending order: what the bar lets through overruns the buffer."""
+    for dtype, piece in ((torch.float32, 16), (torch.bfloat16, 32)):
+        x, t = logits(3, 151936, 12, dtype)
+        place = torch.arange(151936, device="cuda")
+        x = torch.where((place // piece) % 256 < 140, x + 100, x)
+        check(x, t, 32)
+        check(torch.sort(x, dim=1).values, t, 32)
+        check(torch.sort(x, dim=1, descending=True).values, t, 32)
 
 
 def test_captured_and_replayed_on_a_stream():
