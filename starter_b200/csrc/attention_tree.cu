@@ -4,6 +4,7 @@
 // values go to shared memory as floats, a lane scores one key for the warp's four rows (no sum crosses lanes), the online softmax keeps a
 // row's reference in every lane and its sum lane by lane, and for the values the lanes turn to the head's entries.  Everything is float;
 // a result is rounded to the working type once.
+#include "allow_smem.cuh"
 #include "attention_tree.cuh"
 
 #define TP_WARPS 4
@@ -171,9 +172,9 @@ __global__ void __launch_bounds__(TP_WARPS * 32) attention_tree_plain_kernel(con
 template <typename T, int NI>
 static int launch_plain(const TreeArgs& a, int seqs, int max_q_len, cudaStream_t s) {
   const int pitch = ((a.dim + 3) & ~3) + 4, smem = (TP_TILE + 2 * TP_KEYS) * pitch * 4;
-  if (smem > 48 * 1024) {                             // (an attribute of the device the launch goes to)
-    cudaError_t e = cudaFuncSetAttribute(attention_tree_plain_kernel<T, NI>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return (int)e;
+  if (smem > 48 * 1024) {
+    const int e = allow_smem<&attention_tree_plain_kernel<T, NI>>(smem);
+    if (e) return e;
   }
   const int bytes = sizeof(T) == 4 ? 16 : 8;
   const int wide = a.dim % 4 == 0 && (((uintptr_t)a.k_store | (uintptr_t)a.v_store) & (bytes - 1)) == 0;

@@ -9,6 +9,7 @@
 // Places behind the sequence or in front of what a window leaves are copied as zeros, so whatever lies there adds nothing.  A value
 // that is no number must reach the rows that see it and no others, though a weight of zero times it is none: on pages that some row
 // does not see whole such entries are taken out of the tile, and put onto the results of the rows that see them at the end.
+#include "allow_smem.cuh"
 #include "attention_tree.cuh"
 
 #define TM_WARPS 4
@@ -354,10 +355,8 @@ static int launch_rows(const TreeArgs& a, int seqs, int max_q_len, cudaStream_t 
   constexpr int RING = TM_STAGES * 2 * SB_PAGE_TOKENS * D * 2, JOIN = 64 * (D + 8) * 4;
   const int smem = 16 * WR * D * 2 + (RING > JOIN ? RING : JOIN);
   const bool cluster = a.splits > 1 && a.splits <= TM_CLUSTER_MAX;
-  // (an attribute of the device the launch goes to)
-  cudaError_t e = cluster ? cudaFuncSetAttribute(attention_tree_mma_kernel<D, WR, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)
-                          : cudaFuncSetAttribute(attention_tree_mma_kernel<D, WR, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return (int)e;
+  const int e = cluster ? allow_smem<&attention_tree_mma_kernel<D, WR, true>>(smem) : allow_smem<&attention_tree_mma_kernel<D, WR, false>>(smem);
+  if (e) return e;
   const dim3 grid((max_q_len * (a.heads / a.kv_heads) + 16 * WR - 1) / (16 * WR), a.kv_heads * seqs, a.splits);
   if (cluster)
     return launch_dependent_cluster(attention_tree_mma_kernel<D, WR, true>, grid, dim3(TM_THREADS), smem, s, dim3(1, 1, a.splits), a);

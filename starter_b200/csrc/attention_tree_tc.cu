@@ -19,6 +19,7 @@
 // and return.
 #include <cuda.h>
 
+#include "allow_smem.cuh"
 #include "attention_tc.cuh"
 #include "attention_tree.cuh"
 #include "tensor_map.cuh"
@@ -479,9 +480,8 @@ template <int DC> static constexpr int tt_smem() { return (2 * DC + 4 + 3 * DC) 
 
 template <int DC, bool PARTS>
 static int launch_as(const CUtensorMap& mk, const CUtensorMap& mv, const TreeArgs& a, int seqs, int max_q_len, int* status, cudaStream_t s) {
-  // (an attribute of the device the launch goes to)
-  const cudaError_t e = cudaFuncSetAttribute(attention_tree_tc_kernel<DC, PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, tt_smem<DC>());
-  if (e != cudaSuccess) return (int)e;
+  const int e = allow_smem<&attention_tree_tc_kernel<DC, PARTS>>(tt_smem<DC>());
+  if (e) return e;
   const int blocks = (max_q_len * (a.heads / a.kv_heads) + TT_ROWS - 1) / TT_ROWS;
   const dim3 grid(blocks * a.splits, seqs * a.kv_heads);
   if (PARTS) return launch_dependent_cluster(attention_tree_tc_kernel<DC, PARTS>, grid, dim3(TT_THREADS), tt_smem<DC>(), s, dim3(a.splits), mk, mv, a, status);
@@ -503,8 +503,8 @@ void sb_attention_tree_tc_withhold(int step, unsigned long long limit_ns) {
 // How many clusters of `size` of its CTAs, which take an SM each, the current device runs at once, or minus an error.
 int sb_attention_tree_tc_clusters(int size) {
   auto kernel = attention_tree_tc_kernel<2, true>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, tt_smem<2>());
-  if (e != cudaSuccess) return -(int)e;
+  const int set = allow_smem<&attention_tree_tc_kernel<2, true>>(tt_smem<2>());
+  if (set) return -set;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = size;
@@ -516,7 +516,7 @@ int sb_attention_tree_tc_clusters(int size) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   int n = 0;
-  e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
+  const cudaError_t e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
   return e == cudaSuccess ? n : -(int)e;
 }
 

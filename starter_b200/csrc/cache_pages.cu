@@ -9,12 +9,14 @@
 // sequence's nodes, below c; anything else: c is nobody's child).  The nodes on the way lie at places past + path[i] of the
 // sequence; they belong at past + i, and their keys and values go there.
 //
-// Every block walks its sequence's tree itself (a few shared-memory steps of a tree's depth; as a launch of its own it would cost more),
-// then moves a 128-byte column of the keys or values of some (entry, key/value head) pairs: all rows are read to shared memory before
-// any is written, so rows may overlap in any way.
-#define CA_THREADS 128
-#define CA_COLUMN 128                    // bytes of a row a block moves
+// Every block walks its sequence's tree itself (a few shared-memory steps of a tree's depth; a launch of its own would cost more).  A thread then
+// moves one 16-byte column (4 bytes where rows do not allow it) of one entry's keys or values of one key/value head through all rows of the
+// way, eight rows on their way at a time: nodes come after their parents, so path[i] >= i grows with i, and what is written at row i has been
+// read, or is no row of the way.  What bounds it is the chain of the walk, the page numbers, a read and a write: 6 nodes of each of 16
+// sequences in 36 layers (23.6 MB) take 8 us, as blocks that moved 128-byte columns through shared memory one after another 49.
+#define CA_THREADS 256
 #define CA_MAX_NODES 256
+#define CA_FLIGHT 8
 
 struct AcceptArgs {
   uint8_t* store[2];                     // keys, values: [entries, pages, kv_heads, 64, row_bytes]
@@ -36,19 +38,20 @@ struct AcceptArgs {
   int width;
 };
 
+template <typename V>
 __global__ void __launch_bounds__(CA_THREADS) cache_accept_kernel(const AcceptArgs a) {
   __shared__ int child[CA_MAX_NODES], way[CA_MAX_NODES], n_way;
-  __shared__ __align__(16) uint8_t rows[CA_MAX_NODES * CA_COLUMN];
+  __shared__ long long from[CA_MAX_NODES], to[CA_MAX_NODES];   // rows of the first entry and head
   pdl_trigger();
   pdl_wait();
   const int seq = blockIdx.y, tid = threadIdx.x;
   const int start = a.seq_q_start[seq], n = min(a.seq_q_len[seq], min(a.width, CA_MAX_NODES)), past = a.seq_kv_len[seq] - a.seq_q_len[seq];
-  for (int i = tid; i < n; i += CA_THREADS) child[i] = CA_MAX_NODES;
+  const int* pages = a.block_table + (size_t)a.seq_slot[seq] * a.table_stride;
+  // (a thread has one node; its loads do not wait for one another)
+  const int parent = tid < n ? a.parents[start + tid] : -1, token = tid < n ? a.tokens[start + tid] : 0;
+  child[tid] = CA_MAX_NODES;
   __syncthreads();
-  for (int i = tid; i < n; i += CA_THREADS) {
-    const int p = a.parents[start + i];
-    if (p >= 0 && p < i && a.tokens[start + i] == a.drawn[start + p]) atomicMin(&child[p], i);
-  }
+  if (parent >= 0 && parent < tid && token == a.drawn[start + parent]) atomicMin(&child[parent], tid);
   __syncthreads();
   if (tid == 0) {
     int k = 0;
@@ -64,28 +67,30 @@ __global__ void __launch_bounds__(CA_THREADS) cache_accept_kernel(const AcceptAr
     }
     if (tid == 0) a.count[seq] = k;
   }
-  const int* pages = a.block_table + (size_t)a.seq_slot[seq] * a.table_stride;
-  const int columns0 = (a.row_bytes[0] + CA_COLUMN - 1) / CA_COLUMN, columns1 = (a.row_bytes[1] + CA_COLUMN - 1) / CA_COLUMN;
-  const int columns = columns0 + columns1;
-  for (long long job = blockIdx.x; job < (long long)a.pairs * columns; job += gridDim.x) {
+  int first = 0;                                          // the first node that does not stay where it is
+  while (first < k && way[first] == first) ++first;
+  if (first == k) return;
+  if (tid >= first && tid < k) {
+    const int src = past + way[tid], dst = past + tid;
+    from[tid] = (long long)page_row(pages[src / SB_PAGE_TOKENS], 0, src % SB_PAGE_TOKENS, a.kv_heads, 1);
+    to[tid] = (long long)page_row(pages[dst / SB_PAGE_TOKENS], 0, dst % SB_PAGE_TOKENS, a.kv_heads, 1);
+  }
+  __syncthreads();
+  const int columns0 = a.row_bytes[0] / (int)sizeof(V), columns = columns0 + a.row_bytes[1] / (int)sizeof(V);
+  for (long long job = (long long)blockIdx.x * CA_THREADS + tid; job < (long long)a.pairs * columns; job += (long long)gridDim.x * CA_THREADS) {
     const int pair = (int)(job / columns), c = (int)(job - (long long)pair * columns), which = c >= columns0;
-    const int first = (which ? c - columns0 : c) * CA_COLUMN, bytes = min(CA_COLUMN, a.row_bytes[which] - first);
-    const int entry = pair / a.kv_heads, kvh = pair - entry * a.kv_heads;
-    uint8_t* base = a.store[which] + (size_t)entry * a.entry_rows * a.row_bytes[which] + first;
-    auto at = [&](int place) {
-      return base + page_row(pages[place / SB_PAGE_TOKENS], kvh, place % SB_PAGE_TOKENS, a.kv_heads, a.row_bytes[which]);
-    };
-    const int words = bytes / 4;
-    for (int idx = tid; idx < k * words; idx += CA_THREADS) {
-      const int i = idx / words, w = idx - i * words;
-      reinterpret_cast<uint32_t*>(rows)[idx] = reinterpret_cast<const uint32_t*>(at(past + way[i]))[w];
+    const int entry = pair / a.kv_heads, kvh = pair - entry * a.kv_heads, bytes = a.row_bytes[which];
+    uint8_t* base = a.store[which] + ((size_t)entry * a.entry_rows + (size_t)kvh * SB_PAGE_TOKENS) * bytes +
+                    (size_t)(which ? c - columns0 : c) * sizeof(V);
+    for (int i0 = first; i0 < k; i0 += CA_FLIGHT) {
+      V v[CA_FLIGHT];
+#pragma unroll
+      for (int i = 0; i < CA_FLIGHT; ++i)
+        if (i0 + i < k) v[i] = *reinterpret_cast<const V*>(base + (size_t)from[i0 + i] * bytes);
+#pragma unroll
+      for (int i = 0; i < CA_FLIGHT; ++i)
+        if (i0 + i < k) *reinterpret_cast<V*>(base + (size_t)to[i0 + i] * bytes) = v[i];
     }
-    __syncthreads();
-    for (int idx = tid; idx < k * words; idx += CA_THREADS) {
-      const int i = idx / words, w = idx - i * words;
-      if (way[i] != i) reinterpret_cast<uint32_t*>(at(past + i))[w] = reinterpret_cast<const uint32_t*>(rows)[idx];
-    }
-    __syncthreads();
   }
 }
 
@@ -119,10 +124,8 @@ __global__ void __launch_bounds__(CP_THREADS) cache_copy_kernel(const __grid_con
 
 extern "C" {
 
-int sb_cache_accept_max_nodes() { return CA_MAX_NODES; }
-
 // keys and values [entries, pages, kv_heads, 64, row bytes], row bytes multiples of 4; the step's arrays as in attention_tree.cuh;
-// count [seqs], path and taken [seqs, width] or all null.  width: at least every sequence's nodes, at most sb_cache_accept_max_nodes().
+// count [seqs], path and taken [seqs, width] or all null.  width: at least every sequence's nodes, at most 256.
 int sb_cache_accept(void* keys, void* values, int key_bytes, int value_bytes, int entries, int pages, int kv_heads, const int* block_table,
                     int table_stride, const int* seq_slot, const int* seq_q_start, const int* seq_q_len, const int* seq_kv_len, int seqs,
                     const int* tokens, const int* parents, const int* drawn, int* count, int* path, int* taken, int width,
@@ -140,13 +143,14 @@ int sb_cache_accept(void* keys, void* values, int key_bytes, int value_bytes, in
   a.seq_slot = seq_slot; a.seq_q_start = seq_q_start; a.seq_q_len = seq_q_len; a.seq_kv_len = seq_kv_len;
   a.tokens = tokens; a.parents = parents; a.drawn = drawn;
   a.count = count; a.path = path; a.taken = taken; a.width = width;
-  const long long jobs = (long long)a.pairs * ((key_bytes + CA_COLUMN - 1) / CA_COLUMN + (value_bytes + CA_COLUMN - 1) / CA_COLUMN);
-  const long long most = 148 * 8 / seqs > 1 ? 148 * 8 / seqs : 1;
-  return launch_dependent(cache_accept_kernel, dim3((unsigned)(jobs < most ? jobs : most), seqs), dim3(CA_THREADS), 0, s, a);
+  // 16 bytes a thread where rows allow it; one job a thread until the SMs are full
+  const bool wide = (((uintptr_t)keys | (uintptr_t)values | (uintptr_t)key_bytes | (uintptr_t)value_bytes) & 15) == 0;
+  const long long jobs = (long long)a.pairs * ((key_bytes + value_bytes) / (wide ? 16 : 4));
+  const long long blocks = (jobs + CA_THREADS - 1) / CA_THREADS, most = 148 * 8 / seqs > 1 ? 148 * 8 / seqs : 1;
+  const dim3 grid((unsigned)(blocks < most ? blocks : most), seqs);
+  return wide ? launch_dependent(cache_accept_kernel<uint4>, grid, dim3(CA_THREADS), 0, s, a)
+              : launch_dependent(cache_accept_kernel<uint32_t>, grid, dim3(CA_THREADS), 0, s, a);
 }
-
-int sb_cache_copy_max_tensors() { return CP_MAX_TENSORS; }
-int sb_cache_copy_max_pairs() { return CP_MAX_PAIRS; }
 
 // tensors: up to 16 of {address, outer, items, item bytes} (host memory, 64-bit each); pairs: up to 256 of {source, target} (host memory,
 // 32-bit each, every number below each tensor's items; no target is named twice or is a source).

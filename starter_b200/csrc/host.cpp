@@ -166,6 +166,28 @@ PyObject* need(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return PyObject_Vectorcall(refuse, args, n, nullptr);
 }
 
+// fits(t, dtype, sizes...): whether t is a contiguous tensor on the current CUDA device of this type and these sizes (None: any).
+PyObject* fits(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n < 2 || !THPVariable_Check(args[0])) Py_RETURN_FALSE;
+  try {
+    const at::Tensor& t = THPVariable_Unpack(args[0]);
+    if (!t.is_cuda() || t.layout() != at::kStrided || t.dim() != n - 2 || !t.is_contiguous() || t.get_device() != c10::cuda::current_device()) Py_RETURN_FALSE;
+    if (args[1] != Py_None && !(THPDtype_Check(args[1]) && reinterpret_cast<THPDtype*>(args[1])->scalar_type == t.scalar_type())) Py_RETURN_FALSE;
+    for (Py_ssize_t i = 2; i < n; ++i) {
+      if (args[i] == Py_None) continue;
+      const long long want = PyLong_AsLongLong(args[i]);
+      if (want == -1 && PyErr_Occurred()) {
+        PyErr_Clear();
+        Py_RETURN_FALSE;
+      }
+      if (t.size(i - 2) != want) Py_RETURN_FALSE;
+    }
+    Py_RETURN_TRUE;
+  } catch (const std::exception&) {
+    Py_RETURN_FALSE;
+  }
+}
+
 // empty(like, shape, dtype=None): like.new_empty(shape, dtype=dtype).
 PyObject* empty(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if ((n == 2 || n == 3) && THPVariable_Check(args[0]) && PyTuple_Check(args[1]) && PyTuple_GET_SIZE(args[1]) <= 6) {
@@ -343,6 +365,7 @@ PyObject* refuse_with(PyObject*, PyObject* function) {
 
 PyMethodDef methods[] = {
     {"need", (PyCFunction)(void (*)(void))need, METH_FASTCALL, nullptr},
+    {"fits", (PyCFunction)(void (*)(void))fits, METH_FASTCALL, nullptr},
     {"empty", (PyCFunction)(void (*)(void))empty, METH_FASTCALL, nullptr},
     {"product", (PyCFunction)(void (*)(void))product, METH_FASTCALL, nullptr},
     {"block_steps", (PyCFunction)(void (*)(void))block_steps, METH_FASTCALL, nullptr},

@@ -8,6 +8,7 @@
 // written and read again; the scratch is 16 bytes a row and tile.
 //
 // Every wait on an mbarrier gives up after a time limit, raises bit 4 of *status and lets both CTAs drain, free their tensor memory and return.
+#include "allow_smem.cuh"
 #include "cta_pair.cuh"
 #include "logprob_stats.cuh"
 #include "tensor_map.cuh"
@@ -268,9 +269,8 @@ static int sc_bn(int rows, int vocab, int pairs) {
 
 template <bool CAP>
 static int sc_launch(const CUtensorMap& mh, const CUtensorMap& mw, const ScoreArgs& a, int pairs, int smem, cudaStream_t s) {
-  // (an attribute of the device the launch goes to)
-  const cudaError_t e = cudaFuncSetAttribute(score_kernel<CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return (int)e;
+  const int e = allow_smem<&score_kernel<CAP>>(smem);
+  if (e) return e;
   return launch_dependent_cluster(score_kernel<CAP>, dim3(2 * pairs), dim3(PG_THREADS), smem, s, dim3(2, 1, 1), mh, mw, a);
 }
 

@@ -14,6 +14,7 @@
 // rows with 5 110 and 138.)  Entries that are no numbers have no key.
 //
 // A row is shared by the blocks of a cluster, whose results meet in the first one's hands.  What bounds it is reading the logits.
+#include "allow_smem.cuh"
 #include "logprob_stats.cuh"
 
 #define LP_THREADS 256
@@ -319,9 +320,8 @@ static int launch_rows(LogprobArgs a, int first, int rows, int parts, int rest, 
     const int slots = lp_slots<T>(a.vocab, rest ? 1 : parts);
     if (slots > LP_MAX_SLOTS) return -2;
     smem = slots * LP_THREADS * 4;
-    // (an attribute of the device the launch goes to)
-    const cudaError_t e = cudaFuncSetAttribute(token_logprobs_kernel<T, TOP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return (int)e;
+    const int e = allow_smem<&token_logprobs_kernel<T, TOP>>(smem);
+    if (e) return e;
   }
   a.logits = (const T*)a.logits + (size_t)first * a.row_stride;
   a.tokens += first; a.given += first; a.entropy += first;
@@ -345,11 +345,6 @@ static int launch_all(const LogprobArgs& a, int rows, int whole, int parts, cuda
 }
 
 extern "C" {
-
-// The longest rows whose alternatives can be listed: LP_MAX_SLOTS tiles in each of a cluster's blocks.
-long long sb_token_logprobs_max_vocab(int dtype) {
-  return (long long)LP_MAX_CLUSTER * LP_MAX_SLOTS * (LP_TILE_BYTES / (dtype == 0 ? 4 : 2)) - 32;
-}
 
 // logits: [rows, vocab], dtype 0 float, 1 bfloat16, rows `row_stride` entries apart; tokens [rows]; top 0 to 32, at most vocab;
 // given, entropy [rows]; top_value, top_id [rows, top] (null with top 0).  The first `whole` rows have a block each,

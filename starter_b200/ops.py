@@ -9,6 +9,7 @@ refused with an error that names it.
 
 from __future__ import annotations
 
+import array
 import ctypes
 import functools
 
@@ -93,10 +94,10 @@ def _refuse(t, name, dtype=None, ndim=None):
 # launch, are native too (csrc/host.cpp).  The first call of any of them loads the native part and puts it in these names.
 
 def _bind():
-    global _need, _empty, _stream, _product, _block_steps, _mixed_splits
+    global _need, _fits, _empty, _stream, _product, _block_steps, _mixed_splits
     host = build.load_host()
     host.refuse_with(_refuse)
-    _need, _empty, _stream, _product = host.need, host.empty, host.stream, host.product
+    _need, _fits, _empty, _stream, _product = host.need, host.fits, host.empty, host.stream, host.product
     _block_steps, _mixed_splits = host.block_steps, host.mixed_splits
     return host
 
@@ -104,6 +105,13 @@ def _bind():
 def _need(t, name, dtype=None, ndim=None):
     _refuse(t, name, dtype, ndim)          # (what is refused needs no native part)
     _bind()
+
+
+def _fits(t, dtype, *sizes):
+    """Whether ``t`` is a contiguous tensor on the current CUDA device of this type and these sizes (None: any)."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        return False                       # (what is refused needs no native part)
+    return _bind().fits(t, dtype, *sizes)
 
 
 def _empty(like, shape, dtype=None):
@@ -1259,26 +1267,28 @@ def token_logprobs(logits, tokens, top=0, status=None):
     and ``top_ids`` int32 ``[R, top]``.  A negative token stands for none and has the log probability 0; one of V or more has none
     (not a number) and sets bit 1 of ``status``.  Entries of minus infinity have the probability 0; entries that are no numbers make a
     row's results no numbers and are not listed (places left over hold the index -1)."""
-    _refuse_rows(logits, "logits")
-    _need(tokens, "tokens", torch.int32, 1)
-    _here(logits, "logits")
+    if not (_fits(logits, None, None, None) and _fits(tokens, torch.int32, None)):
+        _refuse_rows(logits, "logits")
+        _here(logits, "logits")
+        _need(tokens, "tokens", torch.int32, 1)
+        _here(tokens, "tokens")
     rows, vocab = logits.shape
-    top = int(top)
+    item = logits.element_size()
     if tokens.shape[0] != rows:
         raise KernelError(f"{tokens.shape[0]} tokens for {rows} rows of logits")
-    if not 0 <= top <= min(LOGPROBS_MAX_TOP, vocab):
+    if not 0 <= top <= LOGPROBS_MAX_TOP or top > vocab or vocab == 0:
         raise KernelError(f"{top} alternatives asked for; the kernel lists 0 to {min(LOGPROBS_MAX_TOP, vocab)} of {vocab}")
-    if top and vocab * logits.element_size() > 4 * LOGPROBS_MAX_VOCAB:
-        raise KernelError(f"alternatives of rows of {vocab} entries; {4 * LOGPROBS_MAX_VOCAB // logits.element_size()} are the most")
-    out = _empty(tokens, (2, rows), torch.float32)
-    values, ids = _empty(tokens, (rows, top), torch.float32), _empty(tokens, (rows, top), torch.int32)
+    if top and vocab * item > 4 * LOGPROBS_MAX_VOCAB:
+        raise KernelError(f"alternatives of rows of {vocab} entries; {4 * LOGPROBS_MAX_VOCAB // item} are the most")
+    code = _code(logits.dtype)
+    given, entropy = _empty(tokens, (rows,), torch.float32), _empty(tokens, (rows,), torch.float32)
+    values, ids = _empty(tokens, (rows, top), torch.float32), _empty(tokens, (rows, top))
     if rows:
-        whole, parts = _logprob_plan(rows, vocab * logits.element_size())
+        whole, parts = _logprob_plan(rows, vocab * item)
         rc = _lib("token_logprobs").sb_token_logprobs(
-            _code(logits.dtype), logits, rows, vocab, logits.stride(0), tokens, top, out[0], out[1], values, ids, whole, parts, status,
-            _stream())
+            code, logits, rows, vocab, logits.stride(0), tokens, top, given, entropy, values, ids, whole, parts, status, _stream())
         _check(rc, "token_logprobs", 2 if 0 < whole < rows else 1)
-    return out[0], out[1], values, ids
+    return given, entropy, values, ids
 
 
 def _refuse_rows(t, name):
@@ -1314,7 +1324,7 @@ def linear_logprobs(h, weight, tokens, softcap=None, status=None, withhold=None)
         raise KernelError(f"{tokens.shape[0]} tokens for {rows} rows")
     if vocab == 0 or h.shape[1] == 0:
         raise KernelError(f"a head of shape {tuple(weight.shape)} gives no logits")
-    out = _empty(h, (2, rows), torch.float32)
+    given, entropy = _empty(h, (rows,), torch.float32), _empty(h, (rows,), torch.float32)
     if softcap is not None and not softcap > 0:
         raise KernelError(f"a cap of {softcap}")
     if h.dtype == torch.bfloat16 and rows > TENSOR_CORE_MAX_ROWS and h.shape[1] % 8 == 0 and not (h.data_ptr() | weight.data_ptr()) & 15:
@@ -1322,17 +1332,17 @@ def linear_logprobs(h, weight, tokens, softcap=None, status=None, withhold=None)
         if withhold is not None:
             lib.sb_score_withhold(int(withhold[0]), int(withhold[1]))
         scratch = _empty(h, (lib.sb_score_scratch(rows, vocab),), torch.float32)
-        rc = lib.sb_score(h, weight, tokens, rows, vocab, h.shape[1], float(softcap or 0.0), out[0], out[1], scratch, status, _stream())
+        rc = lib.sb_score(h, weight, tokens, rows, vocab, h.shape[1], float(softcap or 0.0), given, entropy, scratch, status, _stream())
         _refuse_maps(rc, "score's")
         _check(rc, "linear_logprobs", 2)
-        return out[0], out[1]
+        return given, entropy
     chunk = max(1, LOGPROBS_CHUNK_BYTES // (4 * vocab))
     for first in range(0, rows, chunk):
         logits = linear(h[first:first + chunk], weight, out_float=True, status=status)
         if softcap is not None:
             globals()["softcap"](logits, softcap)
-        out[0, first:first + chunk], out[1, first:first + chunk] = token_logprobs(logits, tokens[first:first + chunk], status=status)[:2]
-    return out[0], out[1]
+        given[first:first + chunk], entropy[first:first + chunk] = token_logprobs(logits, tokens[first:first + chunk], status=status)[:2]
+    return given, entropy
 
 
 # ---------------------------------------------------------------------------------------- drafted trees
@@ -1341,16 +1351,26 @@ def linear_logprobs(h, weight, tokens, softcap=None, status=None, withhold=None)
 TREE_MAX_NODES = 256
 
 
-def _tree_step(block_table, seq_slot, seq_q_start, seq_q_len, seq_kv_len, max_q_len):
-    """Check a step's sequence arrays; returns how many sequences there are."""
+def _tree_step_fits(block_table, seq_slot, seq_q_start, seq_q_len, seq_kv_len, max_q_len):
+    """How many sequences a step's arrays describe, or None where something about them is wrong."""
+    if not (_fits(seq_slot, torch.int32, None) and _fits(block_table, torch.int32, None, None) and 1 <= max_q_len <= TREE_MAX_NODES):
+        return None
+    seqs = seq_slot.shape[0]
+    fits = _fits(seq_q_start, torch.int32, seqs) and _fits(seq_q_len, torch.int32, seqs) and _fits(seq_kv_len, torch.int32, seqs)
+    return seqs if fits else None
+
+
+def _refuse_tree_step(block_table, seq_slot, seq_q_start, seq_q_len, seq_kv_len, max_q_len):
+    """What is wrong with a step's arrays."""
     _need(block_table, "block_table", torch.int32, 2)
     for name, t in (("seq_slot", seq_slot), ("seq_q_start", seq_q_start), ("seq_q_len", seq_q_len), ("seq_kv_len", seq_kv_len)):
         _need(t, name, torch.int32, 1)
+        _here(t, name)
         if t.shape[0] != seq_slot.shape[0]:
             raise KernelError(f"{name} has {t.shape[0]} entries for {seq_slot.shape[0]} sequences")
     if not 1 <= max_q_len <= TREE_MAX_NODES:
         raise KernelError(f"trees of {max_q_len} nodes; the kernels take 1 to {TREE_MAX_NODES}")
-    return seq_slot.shape[0]
+    _here(block_table, "block_table")
 
 
 @functools.lru_cache(maxsize=4096)
@@ -1392,33 +1412,22 @@ def attention_tree(q, k_store, v_store, block_table, seq_slot, seq_q_start, seq_
     ``window`` positions before it.  A node that sees nothing gets zeros.  ``max_q_len``: the longest ``seq_q_len`` (at most
     ``TREE_MAX_NODES``; by default what the words hold); rows that belong to no sequence hold nothing.  ``kv_hint``: the longest
     ``seq_kv_len``, by which the keys are cut into parts (wrong, it costs time only)."""
-    _need(q, "q", None, 2)
-    _here(q, "q")
-    code = _code(q.dtype)
-    if kv_heads < 1 or heads % kv_heads:
-        raise KernelError(f"{heads} query heads cannot share {kv_heads} key/value heads")
-    if q.shape[1] != heads * head_dim:
-        raise KernelError(f"q has width {q.shape[1]}, expected {heads * head_dim}")
-    if not 1 <= head_dim <= MAX_HEAD_DIM:
-        raise KernelError(f"head_dim {head_dim} exceeds {MAX_HEAD_DIM}")
-    for store in (k_store, v_store):
-        _need(store, "cache pages", q.dtype, 4)
-        if tuple(store.shape[1:]) != (kv_heads, PAGE_TOKENS, head_dim):
-            raise KernelError(f"cache pages have shape {tuple(store.shape)}")
-    _need(tok_pos, "tok_pos", torch.int32, 1)
-    _need(tree_mask, "tree_mask", torch.int32, 2)
-    words = tree_mask.shape[1]
-    if tok_pos.shape[0] != q.shape[0] or tree_mask.shape[0] != q.shape[0]:
-        raise KernelError(f"{q.shape[0]} rows with {tok_pos.shape[0]} positions and {tree_mask.shape[0]} masks")
     if max_q_len is None:
-        max_q_len = min(32 * words, TREE_MAX_NODES)
-    seqs = _tree_step(block_table, seq_slot, seq_q_start, seq_q_len, seq_kv_len, max_q_len)
-    if 32 * words < max_q_len:
-        raise KernelError(f"masks of {words} words for trees of {max_q_len} nodes")
-    if window is not None and window < 1:
-        raise KernelError(f"a window of {window}")
-    out = _empty(q, q.shape)
-    if q.shape[0] == 0 or seqs == 0:
+        max_q_len = min(32 * tree_mask.shape[1], TREE_MAX_NODES) if isinstance(tree_mask, torch.Tensor) and tree_mask.dim() == 2 else 0
+    seqs, dtype = None, getattr(q, "dtype", None)
+    if _fits(q, None, None, heads * head_dim) and _fits(k_store, dtype, None, kv_heads, PAGE_TOKENS, head_dim) \
+            and _fits(v_store, dtype, None, kv_heads, PAGE_TOKENS, head_dim):
+        rows = q.shape[0]
+        if _fits(tok_pos, torch.int32, rows) and _fits(tree_mask, torch.int32, rows, None):
+            seqs = _tree_step_fits(block_table, seq_slot, seq_q_start, seq_q_len, seq_kv_len, max_q_len)
+    if seqs is None or kv_heads < 1 or heads % kv_heads or not 1 <= head_dim <= MAX_HEAD_DIM or (window is not None and window < 1) \
+            or 32 * tree_mask.shape[1] < max_q_len:
+        _refuse_tree(q, k_store, v_store, tok_pos, tree_mask, heads, kv_heads, head_dim, window)
+        _refuse_tree_step(block_table, seq_slot, seq_q_start, seq_q_len, seq_kv_len, max_q_len)
+        raise KernelError(f"masks of {tree_mask.shape[1]} words for trees of {max_q_len} nodes")
+    code, words = _code(dtype), tree_mask.shape[1]
+    out = _empty(q, (rows, heads * head_dim))
+    if rows == 0 or seqs == 0:
         return out
     group = heads // kv_heads
     aligned = code == 1 and not (q.data_ptr() | k_store.data_ptr() | v_store.data_ptr()) & 15
@@ -1444,8 +1453,8 @@ def attention_tree(q, k_store, v_store, block_table, seq_slot, seq_q_start, seq_
             row_warps, splits = parts
         acc = ml = None
         if splits > 8:
-            acc = _empty(q, (q.shape[0] * heads * splits * head_dim,), torch.float32)
-            ml = _empty(q, (q.shape[0] * heads * splits * 2,), torch.float32)
+            acc = _empty(q, (rows * heads * splits * head_dim,), torch.float32)
+            ml = _empty(q, (rows * heads * splits * 2,), torch.float32)
         rc = _lib("attention_tree_mma").sb_attention_tree_mma(
             q, out, k_store, v_store, block_table, block_table.shape[1], seq_slot, seq_q_start, seq_q_len, seq_kv_len, tok_pos, tree_mask,
             words, seqs, max_q_len, heads, kv_heads, head_dim, scale, int(window or 0), splits, row_warps, acc, ml, _stream())
@@ -1454,13 +1463,37 @@ def attention_tree(q, k_store, v_store, block_table, seq_slot, seq_q_start, seq_
     splits = _tree_plain_splits(-(-max_q_len * group // 16) * kv_heads * seqs, keys)
     acc = ml = None
     if splits > 1:
-        acc = _empty(q, (q.shape[0] * heads * splits * head_dim,), torch.float32)
-        ml = _empty(q, (q.shape[0] * heads * splits * 2,), torch.float32)
+        acc = _empty(q, (rows * heads * splits * head_dim,), torch.float32)
+        ml = _empty(q, (rows * heads * splits * 2,), torch.float32)
     rc = _lib("attention_tree").sb_attention_tree_plain(
         code, q, out, k_store, v_store, block_table, block_table.shape[1], seq_slot, seq_q_start, seq_q_len, seq_kv_len, tok_pos, tree_mask,
         words, seqs, max_q_len, heads, kv_heads, head_dim, scale, int(window or 0), splits, acc, ml, _stream())
     _check(rc, "attention_tree", 2 if splits > 1 else 1)
     return out
+
+
+def _refuse_tree(q, k_store, v_store, tok_pos, tree_mask, heads, kv_heads, head_dim, window):
+    """What is wrong with the operands of ``attention_tree`` beside its step's arrays."""
+    _need(q, "q", None, 2)
+    _code(q.dtype)
+    if kv_heads < 1 or heads % kv_heads:
+        raise KernelError(f"{heads} query heads cannot share {kv_heads} key/value heads")
+    if q.shape[1] != heads * head_dim:
+        raise KernelError(f"q has width {q.shape[1]}, expected {heads * head_dim}")
+    if not 1 <= head_dim <= MAX_HEAD_DIM:
+        raise KernelError(f"head_dim {head_dim} is not 1 to {MAX_HEAD_DIM}")
+    for store in (k_store, v_store):
+        _need(store, "cache pages", q.dtype, 4)
+        if tuple(store.shape[1:]) != (kv_heads, PAGE_TOKENS, head_dim):
+            raise KernelError(f"cache pages have shape {tuple(store.shape)}")
+    _need(tok_pos, "tok_pos", torch.int32, 1)
+    _need(tree_mask, "tree_mask", torch.int32, 2)
+    for name, t in (("q", q), ("cache pages", k_store), ("cache pages", v_store), ("tok_pos", tok_pos), ("tree_mask", tree_mask)):
+        _here(t, name)
+    if tok_pos.shape[0] != q.shape[0] or tree_mask.shape[0] != q.shape[0]:
+        raise KernelError(f"{q.shape[0]} rows with {tok_pos.shape[0]} positions and {tree_mask.shape[0]} masks")
+    if window is not None and window < 1:
+        raise KernelError(f"a window of {window}")
 
 
 def cache_accept(stores, block_table, seq_slot, seq_q_start, seq_q_len, seq_kv_len, tokens, parents, drawn, max_q_len):
@@ -1474,30 +1507,37 @@ def cache_accept(stores, block_table, seq_slot, seq_q_start, seq_q_len, seq_kv_l
     dimension).  Returns int32 ``count`` ``[S]`` (nodes on the way), ``path`` ``[S, max_q_len]`` (which ones, then -1) and ``taken``
     ``[S, max_q_len]`` (what was drawn at each, then -1): the sequence has ``past + count`` tokens now and goes on with
     ``taken[count - 1]``.  ``max_q_len``: the longest ``seq_q_len``, at most ``TREE_MAX_NODES``."""
-    seqs = _tree_step(block_table, seq_slot, seq_q_start, seq_q_len, seq_kv_len, max_q_len)
-    for name, t in (("tokens", tokens), ("parents", parents), ("drawn", drawn)):
-        _need(t, name, torch.int32, 1)
-        if t.shape[0] != tokens.shape[0]:
-            raise KernelError(f"{name} has {t.shape[0]} entries for {tokens.shape[0]} nodes")
-    _here(tokens, "tokens")
+    seqs = _tree_step_fits(block_table, seq_slot, seq_q_start, seq_q_len, seq_kv_len, max_q_len)
+    if seqs is None or not (_fits(tokens, torch.int32, None) and _fits(parents, torch.int32, tokens.shape[0])
+                            and _fits(drawn, torch.int32, tokens.shape[0])):
+        _refuse_tree_step(block_table, seq_slot, seq_q_start, seq_q_len, seq_kv_len, max_q_len)
+        for name, t in (("tokens", tokens), ("parents", parents), ("drawn", drawn)):
+            _need(t, name, torch.int32, 1)
+            _here(t, name)
+            if t.shape[0] != tokens.shape[0]:
+                raise KernelError(f"{name} has {t.shape[0]} entries for {tokens.shape[0]} nodes")
     geometry = []
     for keys, values in stores:
-        for t in (keys, values):
-            _need(t, "cache pages")
-            if t.dim() not in (4, 5) or t.shape[-2] != PAGE_TOKENS or t.shape[:-1] != keys.shape[:-1] or t.numel() == 0:
-                raise KernelError(f"cache pages have shapes {tuple(keys.shape)} and {tuple(values.shape)}")
-        rows = [t.shape[-1] * t.element_size() for t in (keys, values)]
-        if rows[0] % 4 or rows[1] % 4 or keys.data_ptr() % 4 or values.data_ptr() % 4:
-            raise KernelError(f"rows of {rows[0]} and {rows[1]} bytes: the kernel moves words of four")
-        geometry.append((keys, values, rows, keys.shape[0] if keys.dim() == 5 else 1, keys.shape[-4], keys.shape[-3]))
+        shape = getattr(keys, "shape", ())
+        if len(shape) == 4:
+            shape = (1, *shape)
+            keys, values = (t[None] if isinstance(t, torch.Tensor) else t for t in (keys, values))
+        if len(shape) != 5 or not (_fits(keys, None, *shape[:3], PAGE_TOKENS, None) and _fits(values, None, *shape[:3], PAGE_TOKENS, None)):
+            for t in (keys, values):
+                _need(t, "cache pages")
+                _here(t, "cache pages")
+            raise KernelError(f"cache pages have shapes {tuple(keys.shape)} and {tuple(values.shape)}")
+        rows = shape[4] * keys.element_size(), values.shape[4] * values.element_size()
+        if not (rows[0] and rows[1] and shape[0] and shape[1] and shape[2]) or (rows[0] | rows[1] | keys.data_ptr() | values.data_ptr()) & 3:
+            raise KernelError(f"cache pages have shapes {tuple(keys.shape)} and {tuple(values.shape)}, rows of {rows[0]} and {rows[1]} bytes: the kernel "
+                              "moves words of four, one or more of each")
+        geometry.append((keys, values, rows, shape))
     if not geometry:
         raise KernelError("no cache pages are given")
-    count = _empty(tokens, (seqs,))
-    ways = _empty(tokens, (2, seqs, max_q_len))
-    outs = (count, ways[0], ways[1])
+    outs = _empty(tokens, (seqs,)), _empty(tokens, (seqs, max_q_len)), _empty(tokens, (seqs, max_q_len))
     if seqs:
         lib = _lib("cache_pages")
-        for n, (keys, values, rows, entries, pages, kv_heads) in enumerate(geometry):
+        for n, (keys, values, rows, (entries, pages, kv_heads, *_)) in enumerate(geometry):
             count_to, path_to, taken_to = outs if n == 0 else (None, None, None)
             rc = lib.sb_cache_accept(keys, values, rows[0], rows[1], entries, pages, kv_heads, block_table, block_table.shape[1], seq_slot,
                                      seq_q_start, seq_q_len, seq_kv_len, seqs, tokens, parents, drawn, count_to, path_to, taken_to,
@@ -1508,41 +1548,49 @@ def cache_accept(stores, block_table, seq_slot, seq_q_start, seq_q_len, seq_kv_l
 
 # ---------------------------------------------------------------------------------------- pages
 
+#: how many tensors and pairs of pages one launch of ``cache_copy_pages`` takes
+COPY_TENSORS, COPY_PAIRS = 16, 256
+
+
 def cache_copy_pages(stores, source, target, dim=1):
     """Copy page ``source[i]`` to page ``target[i]`` (host integers) in every tensor of ``stores``, for all i at once.
 
     ``stores`` are contiguous tensors of a cache group's storage ``[entries, pages, ...]``; ``dim`` says which dimension counts the pages (0:
     one entry's ``[pages, ...]``, or a state ``[slots, ...]``).  No target may be named twice or be a source: the copies are made in any order."""
-    source, target = [int(p) for p in source], [int(p) for p in target]
-    if len(source) != len(target):
-        raise KernelError(f"{len(source)} pages to copy to {len(target)}")
-    if len(set(target)) < len(target) or set(target) & set(source):
+    pairs, n = array.array("i"), len(target)
+    try:
+        for a, b in zip(source, target):
+            pairs.append(a)
+            pairs.append(b)
+    except (TypeError, OverflowError) as wrong:
+        raise KernelError(f"pages are numbered by integers: {wrong}") from None
+    if len(source) != n:
+        raise KernelError(f"{len(source)} pages to copy to {n}")
+    numbers = set(target)
+    if len(numbers) < n or not numbers.isdisjoint(source):
         raise KernelError("a page is copied to twice, or from and to")
     if dim not in (0, 1):
         raise KernelError(f"pages are counted by the first or the second dimension, not {dim}")
-    described = []
+    low, high = (min(pairs), max(pairs)) if n else (0, -1)
+    described = array.array("q")
     for t in stores:
-        _need(t, "cache pages")
-        _here(t, "cache pages")
-        if t.dim() <= dim:
-            raise KernelError(f"cache pages have shape {tuple(t.shape)}")
-        items = t.shape[dim]
-        if source and not (0 <= min(min(source), min(target)) and max(max(source), max(target)) < items):
+        shape = t.shape if isinstance(t, torch.Tensor) else ()
+        if not _fits(t, None, *(None for _ in shape)) or len(shape) <= dim:
+            _need(t, "cache pages")
+            _here(t, "cache pages")
+            raise KernelError(f"cache pages have shape {tuple(shape)}")
+        outer, items, size = shape[0] if dim else 1, shape[dim], t.numel() * t.element_size()
+        if low < 0 or high >= items:
             raise KernelError(f"a page outside the {items} of the cache")
-        if t.numel() == 0:                       # (a latent's cache keeps no values)
-            continue
-        outer = t.shape[0] if dim else 1
-        described += [t.data_ptr(), outer, items, t.numel() // (outer * items) * t.element_size()]
-    if not source or not described:
+        if size:                                 # (a latent's cache keeps no values)
+            described.extend((t.data_ptr(), outer, items, size // (outer * items)))
+    if not n or not described:
         return
-    lib = _lib("cache_pages")
-    per_tensors, per_pairs = 16, 256
-    pairs = [n for pair in zip(source, target) for n in pair]
-    for t in range(0, len(described), 4 * per_tensors):
-        some = (ctypes.c_longlong * len(described[t:t + 4 * per_tensors]))(*described[t:t + 4 * per_tensors])
-        for p in range(0, len(pairs), 2 * per_pairs):
-            here = (ctypes.c_int * len(pairs[p:p + 2 * per_pairs]))(*pairs[p:p + 2 * per_pairs])
-            rc = lib.sb_cache_copy(ctypes.addressof(some), len(some) // 4, ctypes.addressof(here), len(here) // 2, _stream())
+    entry, stream = _lib("cache_pages").sb_cache_copy, _stream()
+    at_tensors, at_pairs = described.buffer_info()[0], pairs.buffer_info()[0]
+    for t in range(0, len(described) // 4, COPY_TENSORS):
+        for p in range(0, n, COPY_PAIRS):
+            rc = entry(at_tensors + 32 * t, min(COPY_TENSORS, len(described) // 4 - t), at_pairs + 8 * p, min(COPY_PAIRS, n - p), stream)
             _check(rc, "cache_copy_pages")
 
 
