@@ -59,7 +59,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* q_sm = smem;                                   // 2 tiles
   uint8_t* p_sm = q_sm + 2 * Q_BYTES;                     // 2 tiles
-  uint8_t* ring = p_sm + 2 * P_BYTES;                     // buffers 0 and 1: keys of even and odd steps; 2: values
+  uint8_t* ring = p_sm + 2 * P_BYTES;                     // three buffers, in the order of use: K0 K1 V0 K2 V1 K3 V2 ...
   __shared__ uint64_t q_ready[2], full[3], empty[3], s_ready[2], s_free[2], p_ready[2], o_ready[2];
   __shared__ uint32_t tmem_holder;
   __shared__ int abort_flag, sh_low, sh_high, sh_bad;
@@ -114,14 +114,20 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
     n_steps = max(0, min(per, n_steps - first_step));
   }
   volatile int* abort = &abort_flag;
+  // A step's keys and values in the order of copies: copy n goes to buffer n % 3, whose use n / 3 it is.  The values of step i are asked for when S of step
+  // i has been formed, the keys of step i + 2 when PV of step i - 1 has.  (With two buffers for the keys and one for the values a copy's whole way from
+  // memory lay between PV of one step and the next.)
+  auto k_copy = [&](int i) { return i == 0 ? 0 : 2 * i - 1; };
+  auto v_copy = [&](int i) { return i == n_steps - 1 ? 2 * i + 1 : 2 * i + 2; };
 
   if (warp == 8) {
     // ---------------- producer: the whole warp walks the schedule, one elected lane issues the copies
     const bool elected = elect_one();
-    // Keys alternate between buffers 0 and 1 and run a step ahead of the values, which have buffer 2: K0 V0 K1 | K2 V1 | K3 V2 ...
-    auto load = [&](bool is_v, int i) -> bool {
-      const int b = is_v ? 2 : (i & 1), use = is_v ? i : (i >> 1);
-      if (use > 0 && !__all_sync(0xffffffffu, mbar_wait(&empty[b], (use - 1) & 1, abort))) return false;
+    int loads[3] = {0, 0, 0};                             // per buffer: how many copies were started
+    for (int n = 0; n < 2 * n_steps; ++n) {
+      const bool is_v = n == 2 * n_steps - 1 || (n > 0 && n % 2 == 0);
+      const int i = is_v ? (n == 2 * n_steps - 1 ? n_steps - 1 : n / 2 - 1) : (n + 1) / 2, b = n % 3;
+      if (n >= 3 && !__all_sync(0xffffffffu, mbar_wait(&empty[b], (n / 3 - 1) & 1, abort))) break;
       if (elected) mbar_expect_tx(&full[b], DC * SUB);
       const bool withheld = is_v && first_step + i == *(volatile int*)&tc_withhold_step;   // tests only
       for (int half = 0; half < (withheld ? 1 : 2); ++half) {
@@ -129,16 +135,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
         for (int c = 0; c < DC; ++c)
           if (elected) tma_load_2d(ring + b * KV_BYTES + c * SUB + half * 8192, is_v ? &map_v : &map_k, &full[b], c * 64, row);
       }
-      return true;
-    };
-    int loads[3] = {0, 0, 0};                             // per buffer: how many copies were started
-    bool ok = n_steps > 0 && load(false, 0);
-    if (ok) { loads[0]++; ok = load(true, 0); }
-    if (ok) loads[2]++;
-    if (ok && n_steps > 1) { ok = load(false, 1); if (ok) loads[1]++; }
-    for (int i = 1; i < n_steps && ok; ++i) {
-      if (i + 1 < n_steps) { ok = load(false, i + 1); if (ok) loads[(i + 1) & 1]++; }
-      if (ok) { ok = load(true, i); if (ok) loads[2]++; }
+      loads[0] += b == 0; loads[1] += b == 1; loads[2] += b == 2;
     }
     if (*abort && elected) {                              // let the copies in flight land before the block ends
       for (int b = 0; b < 3; ++b) {
@@ -154,11 +151,12 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
       const uint32_t idesc_s = instr_desc(TT_BK, 0), idesc_o = instr_desc(D, 1);
       const uint32_t q_addr = smem_u32(q_sm + t * Q_BYTES), p_addr = smem_u32(p_sm + t * P_BYTES);
       auto issue_s = [&](int buf) {
+        const uint32_t k_addr = smem_u32(ring + buf * KV_BYTES);
         if (elected) {
 #pragma unroll
           for (int k = 0; k < DC * 4; ++k) {
             const uint32_t off = (k >> 2) * SUB + (k & 3) * 32;
-            umma_bf16(tmem_base + t * TT_BK, smem_desc(q_addr + off, 16), smem_desc(smem_u32(ring + buf * KV_BYTES) + off, 16), idesc_s,
+            umma_bf16(tmem_base + t * TT_BK, smem_desc(q_addr + off, 16), smem_desc(k_addr + off, 16), idesc_s,
                       k > 0 ? 1u : 0u);
           }
           umma_commit(&s_ready[t]);
@@ -166,14 +164,15 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
         }
         __syncwarp();
       };
-      auto issue_pv = [&](bool first) {
+      auto issue_pv = [&](bool first, int buf) {
+        const uint32_t v_addr = smem_u32(ring + buf * KV_BYTES);
         if (elected) {
 #pragma unroll
           for (int k = 0; k < TT_BK / 16; ++k)
             umma_bf16(tmem_base + 2 * TT_BK + t * 128, smem_desc(p_addr + (k >> 2) * SUB + (k & 3) * 32, 16),
-                      smem_desc(smem_u32(ring + 2 * KV_BYTES) + k * 2048, SUB), idesc_o, (first && k == 0) ? 0u : 1u);
+                      smem_desc(v_addr + k * 2048, SUB), idesc_o, (first && k == 0) ? 0u : 1u);
           umma_commit(&o_ready[t]);
-          umma_commit(&empty[2]);
+          umma_commit(&empty[buf]);
         }
         __syncwarp();
       };
@@ -190,16 +189,17 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
       // Step i: S of step i+1 as soon as the softmax warps have read S of step i out of tensor memory, then PV of step i when P is written.
       for (int i = 0; i < n_steps && ok; ++i) {
         if (i + 1 < n_steps) {
-          const int kb = (i + 1) & 1;                     // buffer of K(i+1); V(i) is in buffer 2
-          ok = wait2(&full[kb], ((i + 1) >> 1) & 1, &s_free[t], i & 1);
+          const int k = k_copy(i + 1);
+          ok = wait2(&full[k % 3], (k / 3) & 1, &s_free[t], i & 1);
           if (!ok) break;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          issue_s(kb);
+          issue_s(k % 3);
         }
-        ok = wait2(&full[2], i & 1, &p_ready[t], i & 1);
+        const int v = v_copy(i);
+        ok = wait2(&full[v % 3], (v / 3) & 1, &p_ready[t], i & 1);
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        issue_pv(i == 0);
+        issue_pv(i == 0, v % 3);
       }
     }
   } else if (warp < 8 && (warp >> 2) < tiles) {
@@ -247,13 +247,16 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
     for (int i = 0; i < n_steps && ok; ++i) {
       const int j0 = (page_lo + 2 * (first_step + i)) * SB_PAGE_TOKENS;
       const bool edge = j0 + TT_BK > past || j0 < high;   // some row does not see all of the step
+      ok = together(mbar_wait(&s_ready[t], i & 1, abort));
+      if (!ok) break;
       if (edge) {
-        // values that are no numbers leave the tile (both tiles' warps may find the same: they write the same zeros).  These warps may be a
-        // step ahead of the values: only behind PV of the step before does the barrier's parity speak of this step's.
-        ok = together((i == 0 || mbar_wait(&o_ready[t], (i - 1) & 1, abort)) && mbar_wait(&full[2], i & 1, abort));
+        // Values that are no numbers leave the tile (both tiles' warps may find the same: they write the same zeros).  The buffer's use before is over
+        // (it was the keys of S above, or, for the last values, those of two steps before), so its barrier's parity speaks of this one.
+        const int n = v_copy(i);
+        ok = together(mbar_wait(&full[n % 3], (n / 3) & 1, abort));
         if (!ok) break;
         int bad = 0;
-        uint4* v = reinterpret_cast<uint4*>(ring + 2 * KV_BYTES);
+        uint4* v = reinterpret_cast<uint4*>(ring + n % 3 * KV_BYTES);
 #pragma unroll 4
         for (int idx = (warp & 3) * 32 + lane; idx < DC * SUB / 16; idx += 128) {
           const uint4 x = v[idx];
@@ -268,8 +271,6 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
         }
         if (bad) sh_bad = 1;
       }
-      ok = together(mbar_wait(&s_ready[t], i & 1, abort));
-      if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       float sv[64];
       float rs = 0.f, rs_hi = 0.f;                        // the row sum in two halves (packed adds)
