@@ -29,7 +29,6 @@
 #define TT_ROWS (2 * TC_BQ)
 #define TT_MAX_NODES 256
 #define TT_MAX_SPLITS 8
-
 #define TT_WORDS (TT_MAX_NODES / 32)
 // Places j0 .. j0 + 63 as the row sees them: bits[] is its mask, `first` its window's first place (0: no window).
 __device__ __forceinline__ uint64_t tt_view(const uint32_t* bits, int first, int past, int q_len, int j0) {
@@ -44,6 +43,32 @@ __device__ __forceinline__ uint64_t tt_view(const uint32_t* bits, int first, int
   if (end < 64) view &= end > 0 ? (1ull << end) - 1 : 0ull;          // places behind the sequence
   if (hidden > 0) view &= hidden < 64 ? ~0ull << hidden : 0ull;      // cached places in front of the window
   return view;
+}
+// 8 consecutive 32-bit columns of this thread's TMEM lane, there and back (few registers: they run beside a whole row of scores).
+__device__ __forceinline__ void tt_load8(uint32_t taddr, float* v) {
+  uint32_t r[8];
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n\ttcgen05.wait::ld.sync.aligned;"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(taddr) : "memory");
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tt_store8(uint32_t taddr, const float* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+               ::"r"(taddr), "r"(__float_as_uint(v[0])), "r"(__float_as_uint(v[1])), "r"(__float_as_uint(v[2])), "r"(__float_as_uint(v[3])),
+                 "r"(__float_as_uint(v[4])), "r"(__float_as_uint(v[5])), "r"(__float_as_uint(v[6])), "r"(__float_as_uint(v[7])) : "memory");
+}
+// 128 consecutive 32-bit columns of this thread's TMEM lane.
+__device__ __forceinline__ void tt_load128(uint32_t taddr, float* v) {
+  uint32_t r[128];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%128];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%64, %65, %66, %67, %68, %69, %70, %71, %72, %73, %74, %75, %76, %77, %78, %79, %80, %81, %82, %83, %84, %85, %86, %87, %88, %89, %90, %91, %92, %93, %94, %95, %96, %97, %98, %99, %100, %101, %102, %103, %104, %105, %106, %107, %108, %109, %110, %111, %112, %113, %114, %115, %116, %117, %118, %119, %120, %121, %122, %123, %124, %125, %126, %127}, [%129];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63]), "=r"(r[64]), "=r"(r[65]), "=r"(r[66]), "=r"(r[67]), "=r"(r[68]), "=r"(r[69]), "=r"(r[70]), "=r"(r[71]), "=r"(r[72]), "=r"(r[73]), "=r"(r[74]), "=r"(r[75]), "=r"(r[76]), "=r"(r[77]), "=r"(r[78]), "=r"(r[79]), "=r"(r[80]), "=r"(r[81]), "=r"(r[82]), "=r"(r[83]), "=r"(r[84]), "=r"(r[85]), "=r"(r[86]), "=r"(r[87]), "=r"(r[88]), "=r"(r[89]), "=r"(r[90]), "=r"(r[91]), "=r"(r[92]), "=r"(r[93]), "=r"(r[94]), "=r"(r[95]), "=r"(r[96]), "=r"(r[97]), "=r"(r[98]), "=r"(r[99]), "=r"(r[100]), "=r"(r[101]), "=r"(r[102]), "=r"(r[103]), "=r"(r[104]), "=r"(r[105]), "=r"(r[106]), "=r"(r[107]), "=r"(r[108]), "=r"(r[109]), "=r"(r[110]), "=r"(r[111]), "=r"(r[112]), "=r"(r[113]), "=r"(r[114]), "=r"(r[115]), "=r"(r[116]), "=r"(r[117]), "=r"(r[118]), "=r"(r[119]), "=r"(r[120]), "=r"(r[121]), "=r"(r[122]), "=r"(r[123]), "=r"(r[124]), "=r"(r[125]), "=r"(r[126]), "=r"(r[127])
+      : "r"(taddr), "r"(taddr + 64)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 128; ++i) v[i] = __uint_as_float(r[i]);
 }
 __device__ __forceinline__ bool tt_no_number(uint32_t half) { return (half & 0x7f80u) == 0x7f80u; }
 
@@ -60,7 +85,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
   uint8_t* q_sm = smem;                                   // 2 tiles
   uint8_t* p_sm = q_sm + 2 * Q_BYTES;                     // 2 tiles
   uint8_t* ring = p_sm + 2 * P_BYTES;                     // three buffers, in the order of use: K0 K1 V0 K2 V1 K3 V2 ...
-  __shared__ uint64_t q_ready[2], full[3], empty[3], s_ready[2], s_free[2], p_ready[2], o_ready[2];
+  __shared__ uint64_t q_ready[2], full[3], empty[3], s_ready[2], s_free[2], p_ready[2], o_ready[2], apart;
   __shared__ uint32_t tmem_holder;
   __shared__ int abort_flag, sh_low, sh_high, sh_bad;
   float2 row_state = make_float2(-INFINITY, 0.f);         // keys in parts: a row's reference and sum
@@ -87,6 +112,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
       mbar_init(&p_ready[t], 4);
       mbar_init(&o_ready[t], 1);
     }
+    mbar_init(&apart, 1);
     abort_flag = 0;
     sh_low = a.window > 0 ? past : 0;
     sh_high = 0;
@@ -182,6 +208,9 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
         return __all_sync(0xffffffffu, got);
       };
       bool ok = wait2(&q_ready[t], 0, &full[0], 0);
+      // Tile 1 begins half a step behind tile 0: while one tile's warps wait for their scores and hand their weights over, the other's form
+      // exponentials.  (In step with each other both did both at once.)
+      if (ok && t == 1) ok = __all_sync(0xffffffffu, mbar_wait(&apart, 0, abort));
       if (ok) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         issue_s(0);
@@ -272,21 +301,52 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
         if (bad) sh_bad = 1;
       }
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      float sv[64];
-      float rs = 0.f, rs_hi = 0.f;                        // the row sum in two halves (packed adds)
-      // half h of the row of S from tensor memory, masked where the step touches an edge
-      auto load_half = [&](int h) {
-        tmem_load64(tmem_s + h * 64, sv);
-        if (edge) {
+      // The whole row of S first, so that S of the next step can be formed while the exponentials of this one run.
+      float sv[128];
+      tt_load128(tmem_s, sv);
+      if (edge) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
           const uint64_t view = tt_view(bits, first, past, q_len, j0 + h * 64);
           const uint32_t lo = (uint32_t)view, hi = (uint32_t)(view >> 32);
 #pragma unroll
           for (int e = 0; e < 64; ++e)
-            if (!((e < 32 ? lo >> e : hi >> (e - 32)) & 1u)) sv[e] = -INFINITY;
+            if (!((e < 32 ? lo >> e : hi >> (e - 32)) & 1u)) sv[h * 64 + e] = -INFINITY;
         }
-      };
-      uint32_t pk[32];
-      float mx = -INFINITY, m_use = m_ref == -INFINITY ? 0.f : m_ref;
+      }
+      float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int e = 0; e < 128; e += 8)
+#pragma unroll
+        for (int f = 0; f < 4; ++f) m4[f] = fmaxf(fmaxf(m4[f], sv[e + f]), sv[e + f + 4]);
+      const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * a.scale_log2;   // scale_log2 > 0: the maximum commutes with it
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      const bool outgrown = __any_sync(0xffffffffu, mx > m_ref + 8.f);   // also the first keys a row sees (m_ref = -inf)
+      if (lane == 0) mbar_arrive(&s_free[t]);             // S of this step may be overwritten
+      if (i == 0 && threadIdx.x == 0) mbar_arrive(&apart);
+      if (outgrown) {
+        // a new reference: rescale what has been accumulated
+        const float m_new = fmaxf(m_ref, mx);
+        const float alpha = m_ref == -INFINITY ? 1.f : fast_exp2(m_ref - m_new);
+        if (i > 0) {
+          ok = together(mbar_wait(&o_ready[t], (i - 1) & 1, abort));
+          if (!ok) break;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll 1
+          for (int c = 0; c < D; c += 8) {
+            float ov[8];
+            tt_load8(tmem_o + c, ov);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ov[e] *= alpha;
+            tt_store8(tmem_o + c, ov);
+          }
+          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        }
+        l_run *= alpha;
+        m_ref = m_new;
+      }
+      const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
+      float rs = 0.f, rs_hi = 0.f;                        // the row sum in two halves (packed adds)
       // P = exp2(S * scale - m) of 8 keys, rounded to bfloat16: one 16-byte column of the A operand
       auto exp8 = [&](int c, uint32_t* w) {
 #pragma unroll
@@ -299,75 +359,22 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
           w[e] = *reinterpret_cast<const uint32_t*>(&two);
         }
       };
-      auto store8 = [&](int h, int c, const uint32_t* w) {
-        *reinterpret_cast<uint4*>(p_row + h * SUB + ((c ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+      auto store8 = [&](int c, const uint32_t* w) {
+        *reinterpret_cast<uint4*>(p_row + (c >> 3) * SUB + (((c & 7) ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
       };
-      auto s_consumed = [&]() {                           // S of this step may be overwritten
-        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&s_free[t]);
-      };
-      // One pass in the common case: the exponent's reference is the one of the step before.
-      load_half(0);
-#pragma unroll
-      for (int e = 0; e < 64; ++e) mx = fmaxf(mx, sv[e]);
+      uint32_t pk[32];
 #pragma unroll
       for (int c = 0; c < 8; ++c) exp8(c, pk + 4 * c);
-      load_half(1);
+      // P's tile is free once PV of the step before has finished
+      if (i > 0 && !outgrown) ok = together(mbar_wait(&o_ready[t], (i - 1) & 1, abort));
+      if (!ok) break;
 #pragma unroll
-      for (int e = 0; e < 64; ++e) mx = fmaxf(mx, sv[e]);
-      mx *= a.scale_log2;                                 // scale_log2 > 0: the maximum commutes with it
-      const bool outgrown = mx > m_ref + 8.f;             // also the first keys a row sees (m_ref = -inf)
-      if (!__any_sync(0xffffffffu, outgrown)) {
-        s_consumed();
-        // P's tile and O are free once PV of the step before has finished
-        if (i > 0) ok = together(mbar_wait(&o_ready[t], (i - 1) & 1, abort));
-        if (!ok) break;
+      for (int c = 0; c < 8; ++c) store8(c, pk + 4 * c);
 #pragma unroll
-        for (int c = 0; c < 8; ++c) store8(0, c, pk + 4 * c);
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          uint32_t w[4];
-          exp8(c, w);
-          store8(1, c, w);
-        }
-      } else {
-        // a new reference: rescale what has been accumulated, then redo this step's P
-        const float m_new = fmaxf(m_ref, mx);
-        const float alpha = m_ref == -INFINITY ? 1.f : fast_exp2(m_ref - m_new);
-        if (i > 0) {
-          ok = together(mbar_wait(&o_ready[t], (i - 1) & 1, abort));
-          if (!ok) break;
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-#pragma unroll 1
-          for (int c = 0; c < D; c += 32) {
-            float ov[32];
-            tmem_load32(tmem_o + c, ov);
-#pragma unroll
-            for (int e = 0; e < 32; ++e) ov[e] *= alpha;
-            tmem_store32(tmem_o + c, ov);
-          }
-          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-        }
-        l_run *= alpha;
-        m_ref = m_new;
-        m_use = m_ref == -INFINITY ? 0.f : m_ref;
-        rs = 0.f;
-        rs_hi = 0.f;
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          uint32_t w[4];
-          exp8(c, w);
-          store8(1, c, w);
-        }
-        load_half(0);
-        s_consumed();
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          uint32_t w[4];
-          exp8(c, w);
-          store8(0, c, w);
-        }
+      for (int c = 8; c < 16; ++c) {
+        uint32_t w[4];
+        exp8(c, w);
+        store8(c, w);
       }
       l_run += rs + rs_hi;
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
