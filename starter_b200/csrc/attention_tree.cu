@@ -18,6 +18,7 @@ __device__ __forceinline__ void tp_load_rows(float* dst, int pitch, const T* sto
   // n rows of this tile, the others zero: whatever lies in them then adds nothing
   if (wide) {
     const int per = dim / 4;
+#pragma unroll 8
     for (int idx = threadIdx.x; idx < TP_KEYS * per; idx += TP_WARPS * 32) {
       const int r = idx / per, c = (idx - r * per) * 4;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -50,6 +51,8 @@ __global__ void __launch_bounds__(TP_WARPS * 32) attention_tree_plain_kernel(con
   float* q_sm = tp_smem;                              // [16][pitch]
   float* k_sm = q_sm + TP_TILE * pitch;               // [32][pitch]
   float* v_sm = k_sm + TP_KEYS * pitch;               // [32][pitch]
+  __shared__ uint32_t masks[TP_TILE][TREE_MAX_WORDS];
+  __shared__ int sh_low;
   pdl_trigger();
   pdl_wait();
   const int split = blockIdx.z % a.splits, seq = blockIdx.z / a.splits, kvh = blockIdx.y;
@@ -61,30 +64,49 @@ __global__ void __launch_bounds__(TP_WARPS * 32) attention_tree_plain_kernel(con
   const int* pages = a.block_table + (size_t)a.seq_slot[seq] * a.table_stride;
   const T* q = (const T*)a.q;
 
-  for (int idx = threadIdx.x; idx < (TP_TILE + 2 * TP_KEYS) * pitch; idx += TP_WARPS * 32) tp_smem[idx] = 0.f;
-  __syncthreads();
-  for (int idx = threadIdx.x; idx < TP_TILE * a.dim; idx += TP_WARPS * 32) {
-    const int r = idx / a.dim, d = idx - r * a.dim, row = row0 + r;
-    if (row < n_rows)
+  // the tile's queries (rows behind the last look like the last), zeros in the rows' padding
+  if (wide) {
+    const int per = a.dim / 4;
+#pragma unroll 4
+    for (int idx = threadIdx.x; idx < TP_TILE * per; idx += TP_WARPS * 32) {
+      const int r = idx / per, c = (idx - r * per) * 4, row = min(row0 + r, n_rows - 1);
+      const T* src = q + ((size_t)(start + row / group) * a.heads + kvh * group + row % group) * a.dim + c;
+      float4 v;
+      if constexpr (sizeof(T) == 4) {
+        v = *reinterpret_cast<const float4*>(src);
+      } else {
+        const uint2 w = *reinterpret_cast<const uint2*>(src);
+        v = make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
+      }
+      v.x *= a.scale_log2; v.y *= a.scale_log2; v.z *= a.scale_log2; v.w *= a.scale_log2;
+      *reinterpret_cast<float4*>(q_sm + r * pitch + c) = v;
+    }
+  } else {
+    for (int idx = threadIdx.x; idx < (TP_TILE + 2 * TP_KEYS) * pitch; idx += TP_WARPS * 32) tp_smem[idx] = 0.f;
+    __syncthreads();
+    for (int idx = threadIdx.x; idx < TP_TILE * a.dim; idx += TP_WARPS * 32) {
+      const int r = idx / a.dim, d = idx - r * a.dim, row = min(row0 + r, n_rows - 1);
       q_sm[r * pitch + d] = to_f<T>(q[((size_t)(start + row / group) * a.heads + kvh * group + row % group) * a.dim + d]) * a.scale_log2;
+    }
   }
-  // the rows' nodes, positions and masks
-  int pos[TP_ROWS];
-  const uint32_t* bits[TP_ROWS];
-  int lowest = past;                                  // the first place any of the tile's rows sees
+  // the rows' masks and windows
+  int first[TP_ROWS];
 #pragma unroll
   for (int r = 0; r < TP_ROWS; ++r) {
-    const int row = min(row0 + warp * TP_ROWS + r, n_rows - 1), node = start + row / group;
-    pos[r] = a.tok_pos[node];
-    bits[r] = a.mask + (size_t)node * a.words;
+    const int node = min(row0 + warp * TP_ROWS + r, n_rows - 1) / group;
+    first[r] = a.window > 0 ? a.tok_pos[start + node] - a.window + 1 : 0;
+    if (lane < TREE_MAX_WORDS) masks[warp * TP_ROWS + r][lane] = tree_mask_word(a, start, node, lane, q_len, first[r]);
   }
+  if (threadIdx.x == 0) sh_low = a.window > 0 ? past : 0;
+  __syncthreads();
   if (a.window > 0) {
-    lowest = kv_len;
-    for (int row = row0; row < min(row0 + TP_TILE, n_rows); ++row) lowest = min(lowest, a.tok_pos[start + row / group] - a.window + 1);
-    lowest = min(max(lowest, 0), past);
-  } else {
-    lowest = 0;
+    int low = first[0];
+#pragma unroll
+    for (int r = 1; r < TP_ROWS; ++r) low = min(low, first[r]);
+    if (lane == 0) atomicMin(&sh_low, max(low, 0));
+    __syncthreads();
   }
+  const int lowest = sh_low;                          // the first place any of the tile's rows sees
   const int tiles = (kv_len - lowest + TP_KEYS - 1) / TP_KEYS, per = (tiles + a.splits - 1) / a.splits;
   const int begin = lowest + split * per * TP_KEYS, end = min(begin + per * TP_KEYS, kv_len);
 
@@ -120,8 +142,11 @@ __global__ void __launch_bounds__(TP_WARPS * 32) attention_tree_plain_kernel(con
     }
 #pragma unroll
     for (int r = 0; r < TP_ROWS; ++r) {
-      const int j = j0 + lane;
-      if (lane >= n || !tree_sees(a, bits[r], pos[r], past, kv_len, a.tok_pos + start, j)) s[r] = -INFINITY;
+      if (lane >= n) s[r] = -INFINITY;
+      if (j0 + n > past || j0 < first[r]) {           // (what is cached and inside the window is seen)
+        const uint32_t view = (uint32_t)tree_view(masks[warp * TP_ROWS + r], first[r], past, kv_len, j0);
+        if (!((view >> lane) & 1u)) s[r] = -INFINITY;
+      }
       const float m_new = fmaxf(m[r], warp_max(s[r]));
       const float base = m_new == -INFINITY ? 0.f : m_new;
       const float alpha = exp2f(m[r] - base);
@@ -177,7 +202,7 @@ static int launch_plain(const TreeArgs& a, int seqs, int max_q_len, cudaStream_t
     if (e) return e;
   }
   const int bytes = sizeof(T) == 4 ? 16 : 8;
-  const int wide = a.dim % 4 == 0 && (((uintptr_t)a.k_store | (uintptr_t)a.v_store) & (bytes - 1)) == 0;
+  const int wide = a.dim % 4 == 0 && (((uintptr_t)a.q | (uintptr_t)a.k_store | (uintptr_t)a.v_store) & (bytes - 1)) == 0;
   const dim3 grid((max_q_len * (a.heads / a.kv_heads) + TP_TILE - 1) / TP_TILE, a.kv_heads, seqs * a.splits);
   int rc = launch_dependent(attention_tree_plain_kernel<T, NI>, grid, dim3(TP_WARPS * 32), smem, s, a, wide);
   if (rc || a.splits == 1) return rc;

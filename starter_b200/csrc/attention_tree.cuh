@@ -34,12 +34,39 @@ struct TreeArgs {
   float* part_ml;            // [tokens, heads, splits, 2]: reference and sum
 };
 
-// Whether a node at `pos` whose mask stands at `bits` sees place j.
-__device__ __forceinline__ bool tree_sees(const TreeArgs& a, const uint32_t* bits, int pos, int past, int kv_len, const int* node_pos, int j) {
-  if (j < past) return a.window == 0 || j > pos - a.window;
-  const int m = j - past;
-  if (j >= kv_len || m >= 32 * a.words || !((bits[m >> 5] >> (m & 31)) & 1u)) return false;
-  return a.window == 0 || node_pos[m] > pos - a.window;
+#define TREE_MAX_WORDS 8                  // of a mask: 256 nodes
+
+// Which of the places j0 .. j0 + 63 a row sees, as bits: bits[] is its mask (TREE_MAX_WORDS words, without the nodes in front of its window),
+// `first` its window's first place (0: no window).
+__device__ __forceinline__ uint64_t tree_view(const uint32_t* bits, int first, int past, int kv_len, int j0) {
+  uint64_t view = 0;
+  const int m0 = j0 - past;                 // the first place's node, or minus how many cached places come first
+  if (m0 > -64) {
+    const int w = max(m0, 0) >> 5, shift = max(m0, 0) & 31;
+    uint64_t nodes = 0;
+    if (w < TREE_MAX_WORDS) {
+      nodes = (uint64_t)bits[w] | (uint64_t)(w + 1 < TREE_MAX_WORDS ? bits[w + 1] : 0u) << 32;
+      if (shift) nodes = nodes >> shift | (uint64_t)(w + 2 < TREE_MAX_WORDS ? bits[w + 2] : 0u) << (64 - shift);
+    }
+    view = m0 < 0 ? nodes << -m0 | ((1ull << -m0) - 1) : nodes;
+  } else {
+    view = ~0ull;
+  }
+  const int end = kv_len - j0, hidden = min(first, past) - j0;
+  if (end < 64) view &= end > 0 ? (1ull << end) - 1 : 0ull;          // places behind the sequence
+  if (hidden > 0) view &= hidden < 64 ? ~0ull << hidden : 0ull;      // cached places in front of the window
+  return view;
+}
+// Word w of the mask of a sequence's node, without the nodes in front of its window (first: its first place).
+__device__ __forceinline__ uint32_t tree_mask_word(const TreeArgs& a, int start, int node, int w, int q_len, int first) {
+  uint32_t bits = w < a.words ? a.mask[(size_t)(start + node) * a.words + w] : 0u;
+  if (a.window > 0) {
+    for (uint32_t left = bits; left; left &= left - 1) {
+      const int m = 32 * w + __ffs(left) - 1;
+      if (m >= q_len || a.tok_pos[start + m] < first) bits &= ~(left & -left);
+    }
+  }
+  return bits;
 }
 
 // Joins the parts of a (node, head): o = sum_s w_s acc_s / sum_s w_s l_s with w_s = 2^(m_s - max m).  A warp takes a

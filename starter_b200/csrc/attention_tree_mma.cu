@@ -1,6 +1,6 @@
 // Attention of the nodes of drafted trees over the paged cache (see attention_tree.cuh) on mma.sync, in bfloat16: steps whose rows are few.
 //
-// A block takes a tile of 16, 32 or 64 packed rows of one key/value head and walks its part of the sequence's pages.  WR warps own
+// A block takes a tile of 16 or 32 packed rows of one key/value head and walks its part of the sequence's pages.  WR warps own
 // 16 rows each; the 4 / WR warps that own the same rows take a share of a page's 64 keys each.  A page (keys and values) goes to a ring of
 // three shared-memory stages by 16-byte asynchronous copies, two pages ahead, swizzled for ldmatrix; S = Q K^T, the online softmax in
 // float, P rounded to bfloat16 (half a step of 8 bits of each weight, what the prompt kernels do), O += P V.  The warps' results meet in
@@ -80,8 +80,8 @@ __global__ void __launch_bounds__(TM_THREADS) attention_tree_mma_kernel(const Tr
   extern __shared__ __align__(128) uint8_t smem[];
   uint8_t* q_tile = smem;                               // [ROWS][D]
   uint8_t* ring = smem + ROWS * D * 2;                  // stages of (keys, values); the results at the end
-  __shared__ uint32_t sh_mask[ROWS][TM_MAX_NODES / 32]; // of the tile's nodes (at most one a row)
-  __shared__ int sh_pos[ROWS], sh_node_pos[TM_MAX_NODES];
+  __shared__ uint32_t sh_mask[ROWS][TREE_MAX_WORDS];    // of the tile's nodes (at most one a row)
+  __shared__ int sh_first[ROWS];                        // their windows' first places
   __shared__ float sh_m[WK][ROWS], sh_l[WK][ROWS];
   __shared__ float2 cl_ml[ROWS];                        // the block's reference and sum of a row
   __shared__ int sh_low, sh_high, sh_bad;
@@ -96,31 +96,19 @@ __global__ void __launch_bounds__(TM_THREADS) attention_tree_mma_kernel(const Tr
   const int* pages = a.block_table + (size_t)a.seq_slot[seq] * a.table_stride;
   const int node0 = row0 / group, n_nodes = (min(row0 + ROWS, n_rows) - 1) / group - node0 + 1;
 
-  if (tid == 0) { sh_low = a.window > 0 ? past : 0; sh_high = 0; sh_bad = 0; }
-  // ---- the tile's queries (rows behind the last are zero), nodes, masks and positions
-  for (int idx = tid; idx < ROWS * C; idx += TM_THREADS) {
-    const int r = idx / C, c = idx % C, row = row0 + r;
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (row < n_rows)
-      v = *reinterpret_cast<const uint4*>((const bf16*)a.q + ((size_t)(start + row / group) * a.heads + kvh * group + row % group) * D + c * 8);
-    *reinterpret_cast<uint4*>(q_tile + tile_offset<D>(r, c)) = v;
-  }
-  for (int idx = tid; idx < n_nodes * (TM_MAX_NODES / 32); idx += TM_THREADS) {
-    const int n = idx / (TM_MAX_NODES / 32), w = idx % (TM_MAX_NODES / 32);
-    sh_mask[n][w] = w < a.words ? a.mask[(size_t)(start + node0 + n) * a.words + w] : 0u;
-  }
-  __syncthreads();
   if (a.window > 0) {
-    for (int n = tid; n < min(q_len, TM_MAX_NODES); n += TM_THREADS) sh_node_pos[n] = a.tok_pos[start + n];
+    if (tid == 0) { sh_low = past; sh_high = 0; }
+    __syncthreads();
     for (int n = tid; n < n_nodes; n += TM_THREADS) {
-      const int pos = a.tok_pos[start + node0 + n];
-      sh_pos[n] = pos;
-      atomicMin(&sh_low, max(pos - a.window + 1, 0));   // the first place any row sees
-      atomicMax(&sh_high, min(pos - a.window + 1, past));   // from here on every row sees all that is cached
+      const int first = a.tok_pos[start + node0 + n] - a.window + 1;
+      sh_first[n] = first;
+      atomicMin(&sh_low, max(first, 0));                // the first place any row sees
+      atomicMax(&sh_high, min(first, past));            // from here on every row sees all that is cached
     }
     __syncthreads();
   }
-  const int low = sh_low, high = sh_high;
+  if (tid == 0) sh_bad = 0;
+  const int low = a.window > 0 ? sh_low : 0, high = a.window > 0 ? sh_high : 0;
   const int first_page = low / SB_PAGE_TOKENS, end_page = (kv_len + SB_PAGE_TOKENS - 1) / SB_PAGE_TOKENS;
   const int per_split = (end_page - first_page + a.splits - 1) / a.splits;
   const int p_begin = first_page + split * per_split, n_pages = max(min(p_begin + per_split, end_page) - p_begin, 0);
@@ -141,6 +129,22 @@ __global__ void __launch_bounds__(TM_THREADS) attention_tree_mma_kernel(const Tr
 #pragma unroll
   for (int i = 0; i < TM_STAGES - 1; ++i) load_page(i);
 
+  // ---- while those are on their way: the tile's queries (rows behind the last are zero) and its nodes' masks
+#pragma unroll
+  for (int idx0 = 0; idx0 < ROWS * C; idx0 += TM_THREADS) {
+    const int idx = idx0 + tid, r = idx / C, c = idx % C, row = row0 + r;
+    if (idx >= ROWS * C) break;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (row < n_rows)
+      v = *reinterpret_cast<const uint4*>((const bf16*)a.q + ((size_t)(start + row / group) * a.heads + kvh * group + row % group) * D + c * 8);
+    *reinterpret_cast<uint4*>(q_tile + tile_offset<D>(r, c)) = v;
+  }
+  for (int idx = tid; idx < n_nodes * TREE_MAX_WORDS; idx += TM_THREADS) {
+    const int n = idx / TREE_MAX_WORDS, w = idx % TREE_MAX_WORDS;
+    sh_mask[n][w] = tree_mask_word(a, start, node0 + n, w, q_len, a.window > 0 ? sh_first[n] : 0);
+  }
+  __syncthreads();
+
   uint32_t qf[KSTEPS][4];
   {
     const int r = wr * 16 + (lane & 7) + ((lane >> 3) & 1) * 8;
@@ -149,11 +153,11 @@ __global__ void __launch_bounds__(TM_THREADS) attention_tree_mma_kernel(const Tr
       ldmatrix_x4(smem_u32(q_tile + tile_offset<D>(r, 2 * kk + (lane >> 4))), qf[kk][0], qf[kk][1], qf[kk][2], qf[kk][3]);
   }
   // the thread's two rows' nodes in the tile (rows behind the last look like the last)
-  int node[2], pos[2];
+  int node[2], from[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     node[h] = min(row0 + wr * 16 + (lane >> 2) + 8 * h, n_rows - 1) / group - node0;
-    pos[h] = a.window > 0 ? sh_pos[node[h]] : 0;
+    from[h] = a.window > 0 ? sh_first[node[h]] : 0;
   }
   float o[NBLK][4];
 #pragma unroll
@@ -166,7 +170,7 @@ __global__ void __launch_bounds__(TM_THREADS) attention_tree_mma_kernel(const Tr
     __syncthreads();
     const uint8_t* kt = ring + (size_t)(i % TM_STAGES) * STAGE_BYTES;
     uint8_t* vt = const_cast<uint8_t*>(kt) + PAGE_BYTES;
-    const int page_j0 = (p_begin + i) * SB_PAGE_TOKENS, j0 = page_j0 + wk * KEYS;
+    const int page_j0 = (p_begin + i) * SB_PAGE_TOKENS;
     // some row does not see all of the page
     const bool edge = page_j0 + SB_PAGE_TOKENS > past || page_j0 < high;
     if (edge) {
@@ -202,18 +206,26 @@ __global__ void __launch_bounds__(TM_THREADS) attention_tree_mma_kernel(const Tr
     }
     float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-    for (int nb = 0; nb < KBLK; ++nb) {
+    for (int nb = 0; nb < KBLK; ++nb)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float v = s[nb][e] * a.scale_log2;
-        if (edge) {
-          const int j = j0 + nb * 8 + (lane & 3) * 2 + (e & 1), h = e >> 1;
-          if (!tree_sees(a, sh_mask[node[h]], pos[h], past, kv_len, sh_node_pos, j)) v = -INFINITY;
-        }
-        s[nb][e] = v;
-        mx[e >> 1] = fmaxf(mx[e >> 1], v);
+      for (int e = 0; e < 4; ++e) s[nb][e] *= a.scale_log2;
+    if (edge) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        // (shifted so that the thread's own columns of a block of eight keys come first)
+        const uint64_t view = tree_view(sh_mask[node[h]], from[h], past, kv_len, page_j0) >> (wk * KEYS + (lane & 3) * 2);
+        const uint32_t lo = (uint32_t)view, hi = (uint32_t)(view >> 32);
+#pragma unroll
+        for (int nb = 0; nb < KBLK; ++nb)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (!(((nb < 4 ? lo : hi) >> (nb % 4 * 8 + e)) & 1u)) s[nb][2 * h + e] = -INFINITY;
       }
     }
+#pragma unroll
+    for (int nb = 0; nb < KBLK; ++nb)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mx[e >> 1] = fmaxf(mx[e >> 1], s[nb][e]);
     float alpha[2], base[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -299,7 +311,7 @@ __global__ void __launch_bounds__(TM_THREADS) attention_tree_mma_kernel(const Tr
     if (sh_bad) {                                       // what was taken out of the tiles, to those that see it
       const int n = (row0 + r) / group - node0;
       for (int j = p_begin * SB_PAGE_TOKENS; j < min((p_begin + n_pages) * SB_PAGE_TOKENS, kv_len); ++j) {
-        if (!tree_sees(a, sh_mask[n], a.window > 0 ? sh_pos[n] : 0, past, kv_len, sh_node_pos, j)) continue;
+        if (!(tree_view(sh_mask[n], a.window > 0 ? sh_first[n] : 0, past, kv_len, j) & 1ull)) continue;
         const uint32_t v = *reinterpret_cast<const uint32_t*>((const bf16*)a.v_store + page_row(pages[j / SB_PAGE_TOKENS], kvh, j % SB_PAGE_TOKENS, a.kv_heads, D) + d);
         if (no_number(v)) x.x += __uint_as_float(v << 16);
         if (no_number(v >> 16)) x.y += __uint_as_float(v & 0xffff0000u);
@@ -367,13 +379,12 @@ static int launch_rows(const TreeArgs& a, int seqs, int max_q_len, cudaStream_t 
 
 template <int D>
 static int launch(const TreeArgs& a, int seqs, int max_q_len, int row_warps, cudaStream_t s) {
-  return row_warps == 1 ? launch_rows<D, 1>(a, seqs, max_q_len, s) : row_warps == 2 ? launch_rows<D, 2>(a, seqs, max_q_len, s)
-                                                                                    : launch_rows<D, 4>(a, seqs, max_q_len, s);
+  return row_warps == 1 ? launch_rows<D, 1>(a, seqs, max_q_len, s) : launch_rows<D, 2>(a, seqs, max_q_len, s);
 }
 
 extern "C" {
 
-// bfloat16, dim 16, 32, 64 or 128 (-2 otherwise), q and the stores 16-byte aligned; row_warps 1, 2 or 4: tiles of 16, 32 or 64 rows.  Up to eight
+// bfloat16, dim 16, 32, 64 or 128 (-2 otherwise), q and the stores 16-byte aligned; row_warps 1 or 2: tiles of 16 or 32 rows.  Up to eight
 // splits are a cluster; from nine to 32 part_acc and part_ml (see TreeArgs) are needed.  words up to 8.
 int sb_attention_tree_mma(const void* q, void* out, const void* k_store, const void* v_store, const int* block_table, int table_stride,
                           const int* seq_slot, const int* seq_q_start, const int* seq_q_len, const int* seq_kv_len, const int* tok_pos,
@@ -381,12 +392,12 @@ int sb_attention_tree_mma(const void* q, void* out, const void* k_store, const v
                           int splits, int row_warps, float* part_acc, float* part_ml, cudaStream_t s) {
   if (seqs == 0 || max_q_len == 0) return 0;
   if (kv_heads <= 0 || heads % kv_heads || words < 1 || splits < 1 || splits > 32) return -2;
-  if (row_warps != 1 && row_warps != 2 && row_warps != 4) return -2;
+  if (row_warps != 1 && row_warps != 2) return -2;
   if ((long long)seqs * kv_heads > 65535 || max_q_len > TM_MAX_NODES) return -2;
   if (splits > TM_CLUSTER_MAX && (!part_acc || !part_ml)) return -2;
   if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_store | (uintptr_t)v_store) & 15) return -2;
   const TreeArgs a{q, out, k_store, v_store, block_table, table_stride, seq_slot, seq_q_start, seq_q_len, seq_kv_len, tok_pos,
-                   (const uint32_t*)mask, words < TM_MAX_NODES / 32 ? words : TM_MAX_NODES / 32, heads, kv_heads, dim,
+                   (const uint32_t*)mask, words < TREE_MAX_WORDS ? words : TREE_MAX_WORDS, heads, kv_heads, dim,
                    scale * 1.4426950408889634f, window > 0 ? window : 0, splits, part_acc, part_ml};
   switch (dim) {
     case 16: return launch<16>(a, seqs, max_q_len, row_warps, s);

@@ -29,12 +29,11 @@
 #define TT_ROWS (2 * TC_BQ)
 #define TT_MAX_NODES 256
 #define TT_MAX_SPLITS 8
-#define TT_WORDS (TT_MAX_NODES / 32)
-// Places j0 .. j0 + 63 as the row sees them: bits[] is its mask, `first` its window's first place (0: no window).
+// tree_view of a mask in registers: every word is taken by its number.
 __device__ __forceinline__ uint64_t tt_view(const uint32_t* bits, int first, int past, int q_len, int j0) {
   uint64_t view = 0;
 #pragma unroll
-  for (int w = 0; w < TT_WORDS; ++w) {                    // (every word by its number, so that they stay in registers)
+  for (int w = 0; w < TREE_MAX_WORDS; ++w) {
     const int at = past + 32 * w - j0;                    // where its first node stands in the page
     if (at > -32 && at < 64) view |= at >= 0 ? (uint64_t)bits[w] << at : (uint64_t)(bits[w] >> -at);
   }
@@ -258,17 +257,9 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
       if (lane == 0) mbar_arrive(&q_ready[t]);
     }
     const int first = a.window > 0 ? a.tok_pos[start + node] - a.window + 1 : 0;
-    uint32_t bits[TT_WORDS];
+    uint32_t bits[TREE_MAX_WORDS];
 #pragma unroll
-    for (int w = 0; w < TT_WORDS; ++w) {
-      bits[w] = w < a.words ? a.mask[(size_t)(start + node) * a.words + w] : 0u;
-      if (a.window > 0) {                                 // without the nodes in front of the window
-        for (uint32_t left = bits[w]; left; left &= left - 1) {
-          const int m = 32 * w + __ffs(left) - 1;
-          if (m >= q_len || a.tok_pos[start + m] < first) bits[w] &= ~(left & -left);
-        }
-      }
-    }
+    for (int w = 0; w < TREE_MAX_WORDS; ++w) bits[w] = tree_mask_word(a, start, node, w, q_len, first);
     float m_ref = -INFINITY, l_run = 0.f;
     bool ok = true;
     // the whole warp goes on or the whole warp stops: tensor memory is read and written by warps
@@ -547,7 +538,7 @@ int sb_attention_tree_tc(const void* q, void* out, const void* k_store, const vo
   rc = sb_make_map(&mv, v_store, kv_rows, dim, SB_PAGE_TOKENS);
   if (rc) return rc;
   const TreeArgs a{q, out, k_store, v_store, block_table, table_stride, seq_slot, seq_q_start, seq_q_len, seq_kv_len, tok_pos,
-                   (const uint32_t*)mask, words < TT_MAX_NODES / 32 ? words : TT_MAX_NODES / 32, heads, kv_heads, dim,
+                   (const uint32_t*)mask, words < TREE_MAX_WORDS ? words : TREE_MAX_WORDS, heads, kv_heads, dim,
                    scale * 1.4426950408889634f, window > 0 ? window : 0, splits, nullptr, nullptr};
   const bool test_run = next_withhold_step >= 0;
   if (test_run) {

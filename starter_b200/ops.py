@@ -1381,7 +1381,7 @@ def _tree_plain_splits(blocks: int, keys: int) -> int:
 @functools.lru_cache(maxsize=4096)
 def _tree_mma_plan(rows: int, units: int, keys: int) -> tuple:
     """``(row warps, splits)`` of the mma.sync kernel for ``rows`` packed rows of each of ``units`` (sequence, key/value head) pairs."""
-    row_warps = 1 if rows <= 16 else 2 if rows <= 32 else 4
+    row_warps = 1 if units * -(-rows // 16) <= SM_COUNT or rows <= 16 else 2
     blocks = units * -(-rows // (16 * row_warps))
     return row_warps, max(1, min(8, (2 * SM_COUNT) // blocks, -(-keys // PAGE_TOKENS)))
 
