@@ -29,9 +29,7 @@ struct TreeArgs {
   int heads, kv_heads, dim;
   float scale_log2;          // scale * log2(e): exponentials are powers of two
   int window;                // 0: none
-  int splits;                // parts a sequence's keys are cut into
-  float* part_acc;           // [tokens, heads, splits, dim], parts that meet in the second kernel
-  float* part_ml;            // [tokens, heads, splits, 2]: reference and sum
+  int splits;                // parts a sequence's keys are cut into: the blocks of a cluster
 };
 
 #define TREE_MAX_WORDS 8                  // of a mask: 256 nodes
@@ -67,37 +65,4 @@ __device__ __forceinline__ uint32_t tree_mask_word(const TreeArgs& a, int start,
     }
   }
   return bits;
-}
-
-// Joins the parts of a (node, head): o = sum_s w_s acc_s / sum_s w_s l_s with w_s = 2^(m_s - max m).  A warp takes a
-// head of a node; up to 32 parts.
-template <typename T>
-static __global__ void attention_tree_join_kernel(const TreeArgs a) {
-  pdl_trigger();
-  pdl_wait();
-  const int seq = blockIdx.y, node = blockIdx.x;
-  if (node >= a.seq_q_len[seq]) return;
-  const int lane = threadIdx.x & 31;
-  const float* part_ml = a.part_ml;
-  const float* part_acc = a.part_acc;
-  SB_BEHIND_WAIT(part_ml);
-  SB_BEHIND_WAIT(part_acc);
-  const int h = blockIdx.z * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  if (h >= a.heads) return;
-  const size_t at = (size_t)(a.seq_q_start[seq] + node) * a.heads + h, p0 = at * a.splits;
-  // (up to 32 parts: one a lane)
-  const float2 ml = lane < a.splits ? reinterpret_cast<const float2*>(part_ml)[p0 + lane] : make_float2(-INFINITY, 0.f);
-  const float top = warp_max(ml.y != 0.f ? ml.x : -INFINITY);
-  const float w = ml.y != 0.f ? exp2f(ml.x - top) : 0.f, sum = warp_sum(ml.y != 0.f ? ml.y * w : 0.f);
-  const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
-  for (int d0 = 0; d0 < a.dim; d0 += 32) {
-    const int d = d0 + lane;
-    float o = 0.f;
-#pragma unroll 8
-    for (int s = 0; s < a.splits; ++s) {
-      const float x = d < a.dim ? part_acc[(p0 + s) * a.dim + d] : 0.f, f = __shfl_sync(0xffffffffu, w, s);
-      o = f != 0.f ? fmaf(x, f, o) : o;
-    }
-    if (d < a.dim) ((T*)a.out)[at * a.dim + d] = from_f<T>(o * inv);
-  }
 }

@@ -4,7 +4,7 @@
 // 16 rows each; the 4 / WR warps that own the same rows take a share of a page's 64 keys each.  A page (keys and values) goes to a ring of
 // three shared-memory stages by 16-byte asynchronous copies, two pages ahead, swizzled for ldmatrix; S = Q K^T, the online softmax in
 // float, P rounded to bfloat16 (half a step of 8 bits of each weight, what the prompt kernels do), O += P V.  The warps' results meet in
-// shared memory; up to eight parts of a sequence's keys are the blocks of one cluster and meet there, more meet in a second kernel.
+// shared memory; up to eight parts of a sequence's keys are the blocks of one cluster and meet there.
 //
 // Places behind the sequence or in front of what a window leaves are copied as zeros, so whatever lies there adds nothing.  A value
 // that is no number must reach the rows that see it and no others, though a weight of zero times it is none: on pages that some row
@@ -317,16 +317,12 @@ __global__ void __launch_bounds__(TM_THREADS) attention_tree_mma_kernel(const Tr
         if (no_number(v >> 16)) x.y += __uint_as_float(v & 0xffff0000u);
       }
     }
-    if (a.splits == 1) {
-      const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
-      *reinterpret_cast<uint32_t*>((bf16*)a.out + out_at(r) * D + d) = pack_bf16(x.x * inv, x.y * inv);
-    } else if (CLUSTER) {
+    if constexpr (CLUSTER) {
       *reinterpret_cast<float2*>(sh_o + (size_t)r * DP + d) = x;      // (read above by this thread alone)
       if (d == 0) cl_ml[r] = make_float2(top, sum);
     } else {
-      const size_t p = out_at(r) * a.splits + split;
-      *reinterpret_cast<float2*>(a.part_acc + p * D + d) = x;
-      if (d == 0) { a.part_ml[2 * p] = top; a.part_ml[2 * p + 1] = sum; }
+      const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
+      *reinterpret_cast<uint32_t*>((bf16*)a.out + out_at(r) * D + d) = pack_bf16(x.x * inv, x.y * inv);
     }
   }
   if constexpr (CLUSTER) {
@@ -366,15 +362,13 @@ template <int D, int WR>
 static int launch_rows(const TreeArgs& a, int seqs, int max_q_len, cudaStream_t s) {
   constexpr int RING = TM_STAGES * 2 * SB_PAGE_TOKENS * D * 2, JOIN = 64 * (D + 8) * 4;
   const int smem = 16 * WR * D * 2 + (RING > JOIN ? RING : JOIN);
-  const bool cluster = a.splits > 1 && a.splits <= TM_CLUSTER_MAX;
+  const bool cluster = a.splits > 1;
   const int e = cluster ? allow_smem<&attention_tree_mma_kernel<D, WR, true>>(smem) : allow_smem<&attention_tree_mma_kernel<D, WR, false>>(smem);
   if (e) return e;
   const dim3 grid((max_q_len * (a.heads / a.kv_heads) + 16 * WR - 1) / (16 * WR), a.kv_heads * seqs, a.splits);
   if (cluster)
     return launch_dependent_cluster(attention_tree_mma_kernel<D, WR, true>, grid, dim3(TM_THREADS), smem, s, dim3(1, 1, a.splits), a);
-  int rc = launch_dependent(attention_tree_mma_kernel<D, WR, false>, grid, dim3(TM_THREADS), smem, s, a);
-  if (rc || a.splits == 1) return rc;
-  return launch_dependent(attention_tree_join_kernel<bf16>, dim3(max_q_len, seqs, (a.heads + 3) / 4), dim3(128), 0, s, a);
+  return launch_dependent(attention_tree_mma_kernel<D, WR, false>, grid, dim3(TM_THREADS), smem, s, a);
 }
 
 template <int D>
@@ -384,21 +378,19 @@ static int launch(const TreeArgs& a, int seqs, int max_q_len, int row_warps, cud
 
 extern "C" {
 
-// bfloat16, dim 16, 32, 64 or 128 (-2 otherwise), q and the stores 16-byte aligned; row_warps 1 or 2: tiles of 16 or 32 rows.  Up to eight
-// splits are a cluster; from nine to 32 part_acc and part_ml (see TreeArgs) are needed.  words up to 8.
+// bfloat16, dim 16, 32, 64 or 128 (-2 otherwise), q and the stores 16-byte aligned; row_warps 1 or 2: tiles of 16 or 32 rows.  splits 1 to 8.
 int sb_attention_tree_mma(const void* q, void* out, const void* k_store, const void* v_store, const int* block_table, int table_stride,
                           const int* seq_slot, const int* seq_q_start, const int* seq_q_len, const int* seq_kv_len, const int* tok_pos,
                           const void* mask, int words, int seqs, int max_q_len, int heads, int kv_heads, int dim, float scale, int window,
-                          int splits, int row_warps, float* part_acc, float* part_ml, cudaStream_t s) {
+                          int splits, int row_warps, cudaStream_t s) {
   if (seqs == 0 || max_q_len == 0) return 0;
-  if (kv_heads <= 0 || heads % kv_heads || words < 1 || splits < 1 || splits > 32) return -2;
+  if (kv_heads <= 0 || heads % kv_heads || words < 1 || splits < 1 || splits > TM_CLUSTER_MAX) return -2;
   if (row_warps != 1 && row_warps != 2) return -2;
   if ((long long)seqs * kv_heads > 65535 || max_q_len > TM_MAX_NODES) return -2;
-  if (splits > TM_CLUSTER_MAX && (!part_acc || !part_ml)) return -2;
   if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_store | (uintptr_t)v_store) & 15) return -2;
   const TreeArgs a{q, out, k_store, v_store, block_table, table_stride, seq_slot, seq_q_start, seq_q_len, seq_kv_len, tok_pos,
                    (const uint32_t*)mask, words < TREE_MAX_WORDS ? words : TREE_MAX_WORDS, heads, kv_heads, dim,
-                   scale * 1.4426950408889634f, window > 0 ? window : 0, splits, part_acc, part_ml};
+                   scale * 1.4426950408889634f, window > 0 ? window : 0, splits};
   switch (dim) {
     case 16: return launch<16>(a, seqs, max_q_len, row_warps, s);
     case 32: return launch<32>(a, seqs, max_q_len, row_warps, s);

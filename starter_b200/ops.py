@@ -1375,15 +1375,31 @@ def _refuse_tree_step(block_table, seq_slot, seq_q_start, seq_q_len, seq_kv_len,
 
 @functools.lru_cache(maxsize=4096)
 def _tree_plain_splits(blocks: int, keys: int) -> int:
-    return max(1, min(-(-keys // 64), 592 // max(blocks, 1), 32))
+    """Parts a sequence's keys are cut into by the kernel for every type and size."""
+    return max(1, min(8, (3 * SM_COUNT) // blocks, -(-keys // 32)))
 
 
 @functools.lru_cache(maxsize=4096)
-def _tree_mma_plan(rows: int, units: int, keys: int) -> tuple:
-    """``(row warps, splits)`` of the mma.sync kernel for ``rows`` packed rows of each of ``units`` (sequence, key/value head) pairs."""
-    row_warps = 1 if units * -(-rows // 16) <= SM_COUNT or rows <= 16 else 2
+def _tree_mma_plan(rows: int, units: int, keys: int, dim: int) -> tuple:
+    """``(row warps, splits)`` of the mma.sync kernel for ``rows`` packed rows of each of ``units`` (sequence, key/value head) pairs: tiles of 16
+    rows while they are fewer than the SMs, of 32 behind that (a tile reads all keys), and as many parts of the keys as blocks run at once, two
+    an SM (four of heads of up to 64).  Measured (us, heads of 128): 8 pairs of 64 rows behind 1,500 tokens in tiles of 16 / 32 rows, 8
+    parts, 11.2 / 13.3; 128 pairs of 64 rows 44.3 / 42.1; 32 pairs of 16 rows behind 4,096 in 4 / 6 / 8 parts 22.7 / 18.7 / 17.7."""
+    row_warps = 1 if rows <= 16 or units * -(-rows // 16) <= SM_COUNT else 2
     blocks = units * -(-rows // (16 * row_warps))
-    return row_warps, max(1, min(8, (2 * SM_COUNT) // blocks, -(-keys // PAGE_TOKENS)))
+    return row_warps, max(1, min(8, (2 if dim > 64 else 4) * SM_COUNT // blocks, -(-keys // PAGE_TOKENS)))
+
+
+def _tree_on_tmem(rows: int, units: int, keys: int, dim: int) -> bool:
+    """Whether the tcgen05 kernel is the faster one, by the scores a step forms.  Its tiles have 128 rows however few are real, and its
+    blocks take 10 us before the first scores are ready; a score costs it less than half.  Measured (us, mma.sync / tcgen05, heads of 128, scores in
+    millions): 16 pairs of 64 rows behind 1,500 tokens (1.5) 13.4 / 14.0, 32 pairs (3.1) 18.5 / 15.0, 64 pairs behind 500 (2.0) 16.0 / 13.9; 16
+    pairs of 32 rows behind 4,096 (2.1) 15.5 / 18.8, 32 pairs (4.2) 23.5 / 20.7; 128 pairs of 16 rows behind 4,096 (8.4) 42.1 / 47.3; two tiles, 8 pairs of
+    256 rows behind 1,500 (3.1) 19.1 / 24.0, 16 pairs (6.1) 29.3 / 25.2.  Heads of 64, 128 pairs of 32 rows behind 4,096 (16.8) 31.3 / 40.3, 64 pairs of 64
+    rows (16.8) 31.1 / 27.0."""
+    if rows <= (16 if dim > 64 else 32):
+        return False
+    return units * rows * keys > (5_500_000 if rows > 128 else 2_000_000 if units >= 64 else 3_000_000)
 
 
 @functools.lru_cache(maxsize=None)
@@ -1394,9 +1410,12 @@ def _tree_tc_clusters(size: int, device: int) -> int:
     return got
 
 
+@functools.lru_cache(maxsize=4096)
 def _tree_tc_splits(blocks: int, keys: int, device: int) -> int:
-    """How many CTAs share the keys of a block of 256 rows: as many as run at once."""
-    return next((parts for parts in (8, 4, 2) if keys >= 256 * parts and blocks <= _tree_tc_clusters(parts, device)), 1)
+    """How many CTAs share the keys of a block of 256 rows: as many as run at once, with 170 keys or more each.  Measured (us, 1 / 2 / 4 / 8, 64
+    rows of 8 pairs, heads of 64): behind 500 tokens 11.7 / 11.3, behind 1,500 10.7 in 4, 9.7 in 8, behind 4,096 16.3 / 12.2; 64 pairs of 256 rows of 128 behind
+    4,096, which run at once in 2 parts alone, 47.6 in 2, 57.7 in 4."""
+    return next((parts for parts in (8, 4, 2) if keys >= max(800, 170 * parts) and blocks <= _tree_tc_clusters(parts, device)), 1)
 
 
 def attention_tree(q, k_store, v_store, block_table, seq_slot, seq_q_start, seq_q_len, seq_kv_len, tok_pos, tree_mask, heads, kv_heads,
@@ -1434,7 +1453,7 @@ def attention_tree(q, k_store, v_store, block_table, seq_slot, seq_q_start, seq_
     keys = min(kv_hint, window + max_q_len) if window else kv_hint
     if kernel is None:
         kernel = "plain" if not aligned or head_dim not in PREFILL_HEAD_DIMS else "mma"
-        if (kernel == "mma" and head_dim in PREFILL_TC_HEAD_DIMS and scale > 0 and max_q_len * group > 64
+        if (kernel == "mma" and head_dim in PREFILL_TC_HEAD_DIMS and scale > 0 and _tree_on_tmem(max_q_len * group, kv_heads * seqs, keys, head_dim)
                 and k_store.shape[0] * kv_heads * PAGE_TOKENS < 1 << 31):
             kernel = "tcgen05"
     if kernel == "tcgen05":
@@ -1448,27 +1467,17 @@ def attention_tree(q, k_store, v_store, block_table, seq_slot, seq_q_start, seq_
         _check(rc, "attention_tree")
         return out
     if kernel == "mma":
-        row_warps, splits = _tree_mma_plan(max_q_len * group, kv_heads * seqs, keys)
-        if parts is not None:
-            row_warps, splits = parts
-        acc = ml = None
-        if splits > 8:
-            acc = _empty(q, (rows * heads * splits * head_dim,), torch.float32)
-            ml = _empty(q, (rows * heads * splits * 2,), torch.float32)
+        row_warps, splits = parts or _tree_mma_plan(max_q_len * group, kv_heads * seqs, keys, head_dim)
         rc = _lib("attention_tree_mma").sb_attention_tree_mma(
             q, out, k_store, v_store, block_table, block_table.shape[1], seq_slot, seq_q_start, seq_q_len, seq_kv_len, tok_pos, tree_mask,
-            words, seqs, max_q_len, heads, kv_heads, head_dim, scale, int(window or 0), splits, row_warps, acc, ml, _stream())
-        _check(rc, "attention_tree", 2 if splits > 8 else 1)
+            words, seqs, max_q_len, heads, kv_heads, head_dim, scale, int(window or 0), splits, row_warps, _stream())
+        _check(rc, "attention_tree")
         return out
-    splits = _tree_plain_splits(-(-max_q_len * group // 16) * kv_heads * seqs, keys)
-    acc = ml = None
-    if splits > 1:
-        acc = _empty(q, (rows * heads * splits * head_dim,), torch.float32)
-        ml = _empty(q, (rows * heads * splits * 2,), torch.float32)
+    splits = parts or _tree_plain_splits(-(-max_q_len * group // 16) * kv_heads * seqs, keys)
     rc = _lib("attention_tree").sb_attention_tree_plain(
         code, q, out, k_store, v_store, block_table, block_table.shape[1], seq_slot, seq_q_start, seq_q_len, seq_kv_len, tok_pos, tree_mask,
-        words, seqs, max_q_len, heads, kv_heads, head_dim, scale, int(window or 0), splits, acc, ml, _stream())
-    _check(rc, "attention_tree", 2 if splits > 1 else 1)
+        words, seqs, max_q_len, heads, kv_heads, head_dim, scale, int(window or 0), splits, _stream())
+    _check(rc, "attention_tree")
     return out
 
 

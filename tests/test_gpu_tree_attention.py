@@ -281,11 +281,19 @@ def test_keys_in_parts_on_tensor_memory(dim, group, nodes, parts):
 
 
 @pytest.mark.parametrize("dim", [16, 32, 64, 128])
-@pytest.mark.parametrize("parts", [(1, 1), (1, 5), (2, 3), (2, 8), (1, 2), (2, 7), (1, 9), (2, 17), (1, 32)])
+@pytest.mark.parametrize("parts", [(1, 1), (1, 5), (2, 3), (2, 8), (1, 2), (2, 7), (1, 8)])
 def test_keys_in_parts_on_warps(dim, parts):
     sees, depth = trees([21, 1, 0, 40], seed=dim)
     c = Case("bf16", 6, 2, dim, sees, [800, 64, 0, 129], depth, window=300 if parts[1] % 2 else None, seed=dim)
     check(c, ops.attention_tree(**c.on_device(), kernel="mma", parts=parts))
+
+
+@pytest.mark.parametrize("dtype, dim", [("fp32", 128), ("fp32", 200), ("bf16", 96), ("bf16", 7), ("fp32", 18)])
+@pytest.mark.parametrize("parts", [1, 2, 5, 8])
+def test_keys_in_parts_on_the_plain_kernel(dtype, dim, parts):
+    sees, depth = trees([21, 1, 0, 40], seed=dim)
+    c = Case(dtype, 6, 2, dim, sees, [800, 64, 0, 129], depth, window=300 if parts % 2 else None, seed=dim)
+    check(c, ops.attention_tree(**c.on_device(), kernel="plain", parts=parts))
 
 
 @pytest.mark.parametrize("parts", [1, 2])
