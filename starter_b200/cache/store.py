@@ -6,7 +6,9 @@ the page that holds its tokens ``64 * i .. 64 * i + 63``.  Every cache entry of 
 group stores that page at the same index of its own tensor, so one table serves
 all entries.  Groups (entries with the same heads, head size and window) have
 storage of their own.  Next to the pages sits fixed-size state per slot for
-mixers that ask for it; it is zeroed when a sequence opens.
+mixers that ask for it; it is zeroed when a sequence opens.  Sequences that fork
+hold full pages together (a count of holders per shared page); whatever is
+written goes to pages a sequence holds alone.
 
 The reference keeps ``[batch, kv_heads, capacity, head_dim]`` per layer and one
 position for the whole batch (engine/engine.py:856-871); here each sequence has
@@ -150,10 +152,16 @@ class SequenceCache:
         if self.state and length != have:
             raise ValueError(f"the state of slot {slot} stands behind all of its {have} tokens, not behind {length}")
         whole, rest = divmod(length, PAGE_TOKENS)
-        slots = self.slots.take_many(count)
+        slots, fresh = self.slots.take_many(count), []
         try:
             fresh = self.pages.take_many(count if rest else 0)
-        except CacheFull:
+            if fresh:
+                self._copy_items(self.keys + self.values, [self._owned[slot][whole]] * count, fresh, 1)
+            if self.state:
+                self._copy_items(list(self.state.values()), [slot] * count, slots, 0)
+        except Exception:
+            for page in reversed(fresh):
+                self.pages.give_back(page)
             for new in reversed(slots):
                 self.slots.give_back(new)
             raise
@@ -167,10 +175,6 @@ class SequenceCache:
             self._table_host[new, :len(pages)] = pages
             if pages:
                 self._dirty[new] = (0, len(pages))
-        if fresh:
-            self._copy_items(self.keys + self.values, [self._owned[slot][whole]] * count, fresh, 1)
-        if self.state:
-            self._copy_items(list(self.state.values()), [slot] * count, slots, 0)
         return slots
 
     def _copy_items(self, tensors, source, target, dim) -> None:

@@ -271,7 +271,7 @@ class ModelRunner:
         h = model.close(residual, pending, ctx.want_rows)
         tokens = torch.tensor(targets, dtype=torch.int32).to(self.device)
         if top == 0:
-            given, entropy = ops.linear_logprobs(h, model.lm_head, tokens, softcap=model.spec.logit_softcap, status=ctx.status)
+            given, entropy = ops.linear_logprobs(h, model.lm_head, tokens, cap=model.spec.logit_softcap, status=ctx.status)
             return given.tolist(), entropy.tolist(), [[] for _ in targets], [[] for _ in targets]
         parts = []
         rows = max(1, ops.LOGPROBS_CHUNK_BYTES // (4 * model.spec.vocab_size))     # (a long text's logits are not held all at once)

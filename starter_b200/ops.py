@@ -1304,13 +1304,15 @@ def _refuse_rows(t, name):
 
 #: bytes of logits that ``linear_logprobs`` forms at a time where it forms any
 LOGPROBS_CHUNK_BYTES = 256 << 20
+#: rows a launch of the kernel behind it takes: its scratch memory is 16 bytes a row and tile of 128 to 256 vocabulary entries
+LOGPROBS_CHUNK_ROWS = 16384
 
 
-def linear_logprobs(h, weight, tokens, softcap=None, status=None, withhold=None):
+def linear_logprobs(h, weight, tokens, cap=None, status=None, withhold=None):
     """``token_logprobs`` of ``h @ weight.T`` without alternatives: ``(logprob, entropy)``, float32 ``[R]`` each.
 
-    ``h`` ``[R, K]`` are hidden rows behind the final norm, ``weight`` ``[V, K]`` the head, of the same type; ``softcap`` (None: none)
-    caps the logits as ``ops.softcap`` does.  In bfloat16 with more than 128 rows the logits are never in memory (csrc/score_tcgen05.cu);
+    ``h`` ``[R, K]`` are hidden rows behind the final norm, ``weight`` ``[V, K]`` the head, of the same type; ``cap`` (None: none)
+    caps the logits as ``softcap`` does.  In bfloat16 with more than 128 rows the logits are never in memory (csrc/score_tcgen05.cu);
     otherwise they are formed ``LOGPROBS_CHUNK_BYTES`` at a time.  ``withhold = (k_block, limit_ns)`` is for tests of the kernel's give-up
     path: one copy is left out, a wait runs out after ``limit_ns``, bit 4 of ``status`` is set and the result is undefined."""
     _need(h, "h", None, 2)
@@ -1325,22 +1327,26 @@ def linear_logprobs(h, weight, tokens, softcap=None, status=None, withhold=None)
     if vocab == 0 or h.shape[1] == 0:
         raise KernelError(f"a head of shape {tuple(weight.shape)} gives no logits")
     given, entropy = _empty(h, (rows,), torch.float32), _empty(h, (rows,), torch.float32)
-    if softcap is not None and not softcap > 0:
-        raise KernelError(f"a cap of {softcap}")
+    if cap is not None and not cap > 0:
+        raise KernelError(f"a cap of {cap}")
     if h.dtype == torch.bfloat16 and rows > TENSOR_CORE_MAX_ROWS and h.shape[1] % 8 == 0 and not (h.data_ptr() | weight.data_ptr()) & 15:
         lib = _lib("score_tcgen05")
         if withhold is not None:
             lib.sb_score_withhold(int(withhold[0]), int(withhold[1]))
-        scratch = _empty(h, (lib.sb_score_scratch(rows, vocab),), torch.float32)
-        rc = lib.sb_score(h, weight, tokens, rows, vocab, h.shape[1], float(softcap or 0.0), given, entropy, scratch, status, _stream())
-        _refuse_maps(rc, "score's")
-        _check(rc, "linear_logprobs", 2)
+        for first in range(0, rows, LOGPROBS_CHUNK_ROWS):
+            here = min(rows - first, LOGPROBS_CHUNK_ROWS)
+            whole = here == rows
+            scratch = _empty(h, (lib.sb_score_scratch(here, vocab),), torch.float32)
+            rc = lib.sb_score(h if whole else h[first:], weight, tokens if whole else tokens[first:], here, vocab, h.shape[1], float(cap or 0.0),
+                              given if whole else given[first:], entropy if whole else entropy[first:], scratch, status, _stream())
+            _refuse_maps(rc, "score's")
+            _check(rc, "linear_logprobs", 2)
         return given, entropy
     chunk = max(1, LOGPROBS_CHUNK_BYTES // (4 * vocab))
     for first in range(0, rows, chunk):
         logits = linear(h[first:first + chunk], weight, out_float=True, status=status)
-        if softcap is not None:
-            globals()["softcap"](logits, softcap)
+        if cap is not None:
+            softcap(logits, cap)
         given[first:first + chunk], entropy[first:first + chunk] = token_logprobs(logits, tokens[first:first + chunk], status=status)[:2]
     return given, entropy
 
@@ -1430,7 +1436,13 @@ def attention_tree(q, k_store, v_store, block_table, seq_slot, seq_q_start, seq_
     row of ``tree_mask`` (int32 ``[T, words]``, node m is bit m % 32 of word m // 32); with ``window`` only what lies less than
     ``window`` positions before it.  A node that sees nothing gets zeros.  ``max_q_len``: the longest ``seq_q_len`` (at most
     ``TREE_MAX_NODES``; by default what the words hold); rows that belong to no sequence hold nothing.  ``kv_hint``: the longest
-    ``seq_kv_len``, by which the keys are cut into parts (wrong, it costs time only)."""
+    ``seq_kv_len``, by which the kernel and the parts the keys are cut into are chosen (wrong, it costs time only).
+
+    float32 and any head size up to 256 run on the plain kernel (csrc/attention_tree.cu), bfloat16 heads of 16, 32, 64 and 128 on warps
+    (csrc/attention_tree_mma.cu), those of 64 and 128 from some millions of scores on on tcgen05 (csrc/attention_tree_tc.cu).  ``kernel``
+    ("plain", "mma", "tcgen05") and ``parts`` (the splits; for "mma" the row warps and the splits) force a choice.  ``withhold = (step, limit_ns)`` is
+    for tests of the tcgen05 kernel's give-up path: half of the values of that step of 128 keys are not copied, the wait on them runs out after
+    ``limit_ns``, bit 16 of ``status`` is set and the result is undefined."""
     if max_q_len is None:
         max_q_len = min(32 * tree_mask.shape[1], TREE_MAX_NODES) if isinstance(tree_mask, torch.Tensor) and tree_mask.dim() == 2 else 0
     seqs, dtype = None, getattr(q, "dtype", None)

@@ -179,14 +179,15 @@ def test_groups_that_hold_more_than_their_share():
         check(torch.sort(x, dim=1, descending=True).values, t, 32)
 
 
-def test_captured_and_replayed_on_a_stream():
-    x, t = logits(12, 40000, 10)
+@pytest.mark.parametrize("rows", [12, 600, 1300])
+def test_captured_and_replayed_on_a_stream(rows):
+    x, t = logits(rows, 40000, 10)
     graph = torch.cuda.CUDAGraph()
     ops.token_logprobs(x, t, top=5)
     torch.cuda.synchronize()
     with torch.cuda.graph(graph):
         out = ops.token_logprobs(x, t, top=5)
-    y, u = logits(12, 40000, 11)
+    y, u = logits(rows, 40000, 11)
     x.copy_(y), t.copy_(u)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
@@ -220,7 +221,7 @@ def score_case(rows, width, vocab, dtype, seed, size=1.0):
 
 
 def check_score(h, w, t, softcap=None):
-    given, entropy = ops.linear_logprobs(h, w, t, softcap=softcap)
+    given, entropy = ops.linear_logprobs(h, w, t, cap=softcap)
     x = h.double() @ w.double().T
     # a logit of K products summed in 32 bits is off by K 2^-24 of their sizes (tensor cores cut what a sum drops: a whole step,
     # 2^-23); the cap (slope at most 1) adds three roundings of its result
@@ -246,7 +247,7 @@ def test_score_sizes(vocab, width):
     check_score(*score_case(200, width, vocab, torch.bfloat16, vocab + width))
 
 
-@pytest.mark.parametrize("rows, width, vocab", [(1500, 512, 20000), (4100, 128, 9001), (200, 2560, 151936), (140, 130, 700), (260, 17, 300)])
+@pytest.mark.parametrize("rows, width, vocab", [(1500, 512, 20000), (4100, 128, 9001), (200, 2560, 151936), (140, 130, 700), (260, 17, 300), (16385, 64, 300), (33000, 16, 200)])
 def test_score_many(rows, width, vocab):
     check_score(*score_case(rows, width, vocab, torch.bfloat16, rows))
 

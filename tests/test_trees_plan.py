@@ -136,6 +136,21 @@ def test_forks_that_cannot_be():
         c.shorten(5, 0)
 
 
+def test_a_fork_whose_copy_fails_changes_nothing(monkeypatch):
+    c = make_cache(state=True)
+    slot = grown(c, 70)
+    free = (c.slots.free_count, c.pages.free_count)
+
+    def broken(tensors, source, target, dim):
+        raise RuntimeError("no")
+
+    monkeypatch.setattr(c, "_copy_items", broken)
+    with pytest.raises(RuntimeError):
+        c.fork(slot, 2)
+    assert (c.slots.free_count, c.pages.free_count) == free and not c._holders and c.lengths[slot] == 70
+    c.check()
+
+
 def test_a_state_is_copied_and_does_not_go_back():
     c = make_cache(state=True)
     slot = grown(c, 70)
