@@ -247,7 +247,7 @@ __global__ void __launch_bounds__(TP_THREADS) attention_tree_plain_kernel(const 
       const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
       ((T*)a.out)[((size_t)(start + row / group) * a.heads + kvh * group + row % group) * a.dim + d] = from_f<T>(o * inv);
     }
-    tp_cluster_barrier();                             // nobody leaves while its shared memory is read
+    tree_cluster_leave();
   } else
 #pragma unroll
   for (int r = 0; r < TP_ROWS; ++r) {

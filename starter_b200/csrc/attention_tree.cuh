@@ -32,6 +32,15 @@ struct TreeArgs {
   int splits;                // parts a sequence's keys are cut into: the blocks of a cluster
 };
 
+// The end of a cluster whose blocks have read from one another: nobody leaves before all have what they read.  (Relaxed: what a thread read it has used
+// by now, and a release would wait for its results' way to memory.)
+__device__ __forceinline__ void tree_cluster_leave() {
+  __syncwarp();                            // (.aligned: a whole warp at once)
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 #define TREE_MAX_WORDS 8                  // of a mask: 256 nodes
 
 // Which of the places j0 .. j0 + 63 a row sees, as bits: bits[] is its mask (TREE_MAX_WORDS words, without the nodes in front of its window),

@@ -293,35 +293,52 @@ __global__ void __launch_bounds__(TM_THREADS) attention_tree_mma_kernel(const Tr
     const int row = row0 + r;
     return ((size_t)(start + row / group) * a.heads + kvh * group + row % group);
   };
-  for (int idx = tid; idx < rows_here * (D / 2); idx += TM_THREADS) {
-    const int r = idx / (D / 2), d = (idx - r * (D / 2)) * 2;
+  if (tid < rows_here) {                                // the weights the warps' parts of a row have in it (negative: a part without keys)
     float top = -INFINITY, sum = 0.f;
-    float2 x = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int w = 0; w < WK; ++w) top = fmaxf(top, sh_l[w][r] != 0.f ? sh_m[w][r] : -INFINITY);
+    for (int w = 0; w < WK; ++w) top = fmaxf(top, sh_l[w][tid] != 0.f ? sh_m[w][tid] : -INFINITY);
 #pragma unroll
     for (int w = 0; w < WK; ++w) {
-      if (sh_l[w][r] == 0.f) continue;
-      const float f = WK == 1 ? 1.f : fast_exp2(sh_m[w][r] - top);
-      const float2 y = *reinterpret_cast<const float2*>(sh_o + ((size_t)w * ROWS + r) * DP + d);
-      sum = fmaf(sh_l[w][r], f, sum);
-      x.x = fmaf(y.x, f, x.x);
-      x.y = fmaf(y.y, f, x.y);
+      const float l = sh_l[w][tid], f = l == 0.f ? -1.f : WK == 1 ? 1.f : fast_exp2(sh_m[w][tid] - top);
+      if (l != 0.f) sum = fmaf(l, f, sum);
+      sh_m[w][tid] = f;
     }
-    if (sh_bad) {                                       // what was taken out of the tiles, to those that see it
-      const int n = (row0 + r) / group - node0;
+    cl_ml[tid] = make_float2(top, sum);
+  }
+  __syncthreads();
+  // (every entry of a row is one thread's from here to the end of the block)
+#pragma unroll 4
+  for (int idx = tid; idx < rows_here * (D / 2); idx += TM_THREADS) {
+    const int r = idx / (D / 2), d = (idx - r * (D / 2)) * 2;
+    float2 x = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < WK; ++w) {
+      const float f = sh_m[w][r];
+      const float2 y = *reinterpret_cast<const float2*>(sh_o + ((size_t)w * ROWS + r) * DP + d);
+      // (a weight below zero is not, one that is no number is)
+      x.x = f < 0.f ? x.x : fmaf(y.x, f, x.x);
+      x.y = f < 0.f ? x.y : fmaf(y.y, f, x.y);
+    }
+    *reinterpret_cast<float2*>(sh_o + (size_t)r * DP + d) = x;
+  }
+  if (sh_bad) {                                         // what was taken out of the tiles, to the rows that see it
+#pragma unroll 1
+    for (int idx = tid; idx < rows_here * (D / 2); idx += TM_THREADS) {
+      const int r = idx / (D / 2), d = (idx - r * (D / 2)) * 2, n = (row0 + r) / group - node0;
+      float2* x = reinterpret_cast<float2*>(sh_o + (size_t)r * DP + d);
       for (int j = p_begin * SB_PAGE_TOKENS; j < min((p_begin + n_pages) * SB_PAGE_TOKENS, kv_len); ++j) {
         if (!(tree_view(sh_mask[n], a.window > 0 ? sh_first[n] : 0, past, kv_len, j) & 1ull)) continue;
         const uint32_t v = *reinterpret_cast<const uint32_t*>((const bf16*)a.v_store + page_row(pages[j / SB_PAGE_TOKENS], kvh, j % SB_PAGE_TOKENS, a.kv_heads, D) + d);
-        if (no_number(v)) x.x += __uint_as_float(v << 16);
-        if (no_number(v >> 16)) x.y += __uint_as_float(v & 0xffff0000u);
+        if (no_number(v)) x->x += __uint_as_float(v << 16);
+        if (no_number(v >> 16)) x->y += __uint_as_float(v & 0xffff0000u);
       }
     }
-    if constexpr (CLUSTER) {
-      *reinterpret_cast<float2*>(sh_o + (size_t)r * DP + d) = x;      // (read above by this thread alone)
-      if (d == 0) cl_ml[r] = make_float2(top, sum);
-    } else {
-      const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
+  }
+  if constexpr (!CLUSTER) {
+    for (int idx = tid; idx < rows_here * (D / 2); idx += TM_THREADS) {
+      const int r = idx / (D / 2), d = (idx - r * (D / 2)) * 2;
+      const float sum = cl_ml[r].y, inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
+      const float2 x = *reinterpret_cast<const float2*>(sh_o + (size_t)r * DP + d);
       *reinterpret_cast<uint32_t*>((bf16*)a.out + out_at(r) * D + d) = pack_bf16(x.x * inv, x.y * inv);
     }
   }
@@ -354,7 +371,7 @@ __global__ void __launch_bounds__(TM_THREADS) attention_tree_mma_kernel(const Tr
       const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
       *reinterpret_cast<uint32_t*>((bf16*)a.out + out_at(r) * D + d) = pack_bf16(y.x * inv, y.y * inv);
     }
-    cluster_barrier();                                  // nobody leaves while its shared memory is read
+    tree_cluster_leave();
   }
 }
 

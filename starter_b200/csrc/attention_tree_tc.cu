@@ -463,7 +463,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
         }
       }
     }
-    cluster_barrier();                                    // nobody leaves while others read from it
+    tree_cluster_leave();
   }
   __syncthreads();
   if (warp == 9) {

@@ -65,9 +65,21 @@ __device__ __forceinline__ Key lp_peer_key(uint32_t a) {
   asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
   return v;
 }
-__device__ __forceinline__ void lp_cluster_barrier() {
+__device__ __forceinline__ void lp_cluster_arrive() {
   __syncwarp();                    // (.aligned: a whole warp at once)
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void lp_cluster_wait() {
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The parts of `lanes` lanes, a power of two, joined: in every one of them.
+__device__ __forceinline__ void lp_join_lanes(Stats& st, int lanes) {
+#pragma unroll
+  for (int o = lanes / 2; o > 0; o >>= 1) {
+    const Stats other{__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.l, o), __shfl_xor_sync(0xffffffffu, st.t, o)};
+    st = lp_join(st, other);
+  }
 }
 
 // 32 bytes on their boundary, which are not needed again.
@@ -153,15 +165,19 @@ __global__ void __launch_bounds__(LP_THREADS, 4) token_logprobs_kernel(const Log
     slot = next;
   }
 
-  // The `want` best of the buffer's `count` keys to list, in order (zeros behind them).  Every thread, between barriers.
+  // The `want` best of the buffer's `count` keys to list, in order (zeros behind them); four lanes count for a key.  Every thread, between barriers.
+  const int quad = threadIdx.x / 4, in_quad = threadIdx.x & 3;
+  auto over_quad = [&](int n) { n += __shfl_xor_sync(0xffffffffu, n, 1); return n + __shfl_xor_sync(0xffffffffu, n, 2); };
   auto rank = [&](int count, int want) {
     if (threadIdx.x <= LP_MAX_TOP) list[threadIdx.x] = 0;
     __syncthreads();
-    for (int i = threadIdx.x; i < count; i += LP_THREADS) {
-      const Key mine = buffer[i];
+    for (int i0 = 0; i0 < count; i0 += LP_QUADS) {
+      const Key mine = i0 + quad < count ? buffer[i0 + quad] : 0;
       int above = 0;
-      for (int j = 0; j < count; ++j) above += buffer[j] > mine;
-      if (above < want) list[above] = mine;
+#pragma unroll 4
+      for (int j = in_quad; j < count; j += 4) above += buffer[j] > mine;
+      above = over_quad(above);
+      if (in_quad == 0 && mine && above < want) list[above] = mine;
     }
     __syncthreads();
   };
@@ -175,16 +191,17 @@ __global__ void __launch_bounds__(LP_THREADS, 4) token_logprobs_kernel(const Log
       for (int s = 0; s < slots; ++s) best = max(best, group_key(s));
 #pragma unroll
     for (int o = 1; o < 4; o <<= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-    if ((lane & 3) == 0) quad_best[threadIdx.x / 4] = best;
+    if (in_quad == 0) quad_best[quad] = best;
     if (threadIdx.x == 0) sh_count = 0;
     __syncthreads();
-    if (threadIdx.x < LP_QUADS) {
-      const Key mine = quad_best[threadIdx.x];
-      int above = 0;
-#pragma unroll 8
-      for (int j = 0; j < LP_QUADS; ++j) above += quad_best[j] > mine || (quad_best[j] == mine && j < threadIdx.x);
-      if (above == want - 1) sh_bar = mine;               // `want` groups reach it (or there are not that many, and it is 0)
+    int better = 0;
+#pragma unroll
+    for (int n = 0; n < LP_QUADS / 4; ++n) {
+      const int j = 4 * n + in_quad;
+      better += quad_best[j] > best || (quad_best[j] == best && j < quad);
     }
+    better = over_quad(better);
+    if (in_quad == 0 && better == want - 1) sh_bar = best;   // `want` groups reach it (or there are not that many, and it is 0)
     __syncthreads();
     {
       const Key bar = sh_bar;
@@ -241,46 +258,44 @@ __global__ void __launch_bounds__(LP_THREADS, 4) token_logprobs_kernel(const Log
   }
 
   // the lanes', then the warps', then the blocks' parts
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const Stats other{__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.l, o), __shfl_xor_sync(0xffffffffu, st.t, o)};
-    st = lp_join(st, other);
-  }
+  lp_join_lanes(st, 32);
   if (lane == 0) { sh_stats[warp][0] = st.m; sh_stats[warp][1] = st.l; sh_stats[warp][2] = st.t; }
+  if (threadIdx.x == 0) sh_count = 0;
   __syncthreads();
   if (warp == 0) {
-    st = lane < LP_WARPS ? Stats{sh_stats[lane][0], sh_stats[lane][1], sh_stats[lane][2]} : Stats{-INFINITY, 0.f, 0.f};
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const Stats other{__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.l, o), __shfl_xor_sync(0xffffffffu, st.t, o)};
-      st = lp_join(st, other);
-    }
+    const int w = lane % LP_WARPS;
+    st = Stats{sh_stats[w][0], sh_stats[w][1], sh_stats[w][2]};
+    lp_join_lanes(st, LP_WARPS);
   }
   if (parts > 1) {
-    if (warp == 0) {
-      if (lane == 0) { cl_stats[0] = st.m; cl_stats[1] = st.l; cl_stats[2] = st.t; }
-    }
-    __syncthreads();
-    lp_cluster_barrier();
+    if (threadIdx.x == 0) { cl_stats[0] = st.m; cl_stats[1] = st.l; cl_stats[2] = st.t; }
+    lp_cluster_arrive();
+    lp_cluster_wait();
     if (part == 0) {
       if (TOP) {
-        for (int i = threadIdx.x; i < parts * a.top; i += LP_THREADS) buffer[i] = lp_peer_key(lp_peer(&list[i % a.top], i / a.top));
-        __syncthreads();
+        // Of the blocks' lists, each in order, what reaches the least of their n-th entries, n parts >= top: at least `top` do.
+        const int n = (a.top + parts - 1) / parts - 1;
+        Key mine = 0, bar = ~0ull;
+        if (threadIdx.x < parts * a.top) mine = lp_peer_key(lp_peer(&list[threadIdx.x % a.top], threadIdx.x / a.top));
+        for (int p = 0; p < parts; ++p) bar = min(bar, lp_peer_key(lp_peer(&list[n], p)));
+        if (mine && mine >= bar) buffer[atomicAdd(&sh_count, 1)] = mine;
       }
       if (warp == 0) {
-        st = Stats{-INFINITY, 0.f, 0.f};
-        if (lane < parts)
-          st = Stats{lp_peer_load(lp_peer(&cl_stats[0], lane)), lp_peer_load(lp_peer(&cl_stats[1], lane)), lp_peer_load(lp_peer(&cl_stats[2], lane))};
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-          const Stats other{__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.l, o), __shfl_xor_sync(0xffffffffu, st.t, o)};
-          st = lp_join(st, other);
-        }
+        const int p = lane % parts;
+        st = Stats{lp_peer_load(lp_peer(&cl_stats[0], p)), lp_peer_load(lp_peer(&cl_stats[1], p)), lp_peer_load(lp_peer(&cl_stats[2], p))};
+        lp_join_lanes(st, parts);
       }
     }
-    lp_cluster_barrier();                                 // nobody leaves while it is read
-    if (part) return;
-    if (TOP) rank(parts * a.top, a.top);
+    lp_cluster_arrive();
+    if (part) {
+      lp_cluster_wait();                                  // nobody leaves while it is read
+      return;
+    }
+    if (TOP) {
+      __syncthreads();
+      rank(sh_count, a.top);
+    }
+    lp_cluster_wait();
   }
   if (warp == 0) {
     if (rest) pdl_wait();

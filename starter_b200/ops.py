@@ -1318,7 +1318,8 @@ def linear_logprobs(h, weight, tokens, cap=None, status=None, withhold=None):
     _need(h, "h", None, 2)
     _need(weight, "weight", h.dtype, 2)
     _need(tokens, "tokens", torch.int32, 1)
-    _here(h, "h")
+    for name, t in (("h", h), ("weight", weight), ("tokens", tokens)):
+        _here(t, name)
     rows, vocab = h.shape[0], weight.shape[0]
     if weight.shape[1] != h.shape[1]:
         raise KernelError(f"weight {tuple(weight.shape)} does not take inputs of width {h.shape[1]}")
