@@ -306,20 +306,28 @@ __global__ void __launch_bounds__(TM_THREADS) attention_tree_mma_kernel(const Tr
     cl_ml[tid] = make_float2(top, sum);
   }
   __syncthreads();
-  // (every entry of a row is one thread's from here to the end of the block)
-#pragma unroll 4
-  for (int idx = tid; idx < rows_here * (D / 2); idx += TM_THREADS) {
-    const int r = idx / (D / 2), d = (idx - r * (D / 2)) * 2;
-    float2 x = make_float2(0.f, 0.f);
+  // (every entry of a row is one thread's from here to the end of the block; loads in front of stores, which they could be for all the compiler knows)
+  constexpr int FLIGHT = 4;
+  for (int idx0 = tid; idx0 < rows_here * (D / 2); idx0 += FLIGHT * TM_THREADS) {
+    float2 x[FLIGHT];
 #pragma unroll
-    for (int w = 0; w < WK; ++w) {
-      const float f = sh_m[w][r];
-      const float2 y = *reinterpret_cast<const float2*>(sh_o + ((size_t)w * ROWS + r) * DP + d);
-      // (a weight below zero is not, one that is no number is)
-      x.x = f < 0.f ? x.x : fmaf(y.x, f, x.x);
-      x.y = f < 0.f ? x.y : fmaf(y.y, f, x.y);
+    for (int u = 0; u < FLIGHT; ++u) {
+      const int idx = idx0 + u * TM_THREADS, r = min(idx / (D / 2), ROWS - 1), d = idx % (D / 2) * 2;
+      x[u] = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < WK; ++w) {
+        const float f = sh_m[w][r];
+        const float2 y = *reinterpret_cast<const float2*>(sh_o + ((size_t)w * ROWS + r) * DP + d);
+        // (a weight below zero is not, one that is no number is)
+        x[u].x = f < 0.f ? x[u].x : fmaf(y.x, f, x[u].x);
+        x[u].y = f < 0.f ? x[u].y : fmaf(y.y, f, x[u].y);
+      }
     }
-    *reinterpret_cast<float2*>(sh_o + (size_t)r * DP + d) = x;
+#pragma unroll
+    for (int u = 0; u < FLIGHT; ++u) {
+      const int idx = idx0 + u * TM_THREADS, r = idx / (D / 2), d = idx % (D / 2) * 2;
+      if (r < rows_here) *reinterpret_cast<float2*>(sh_o + (size_t)r * DP + d) = x[u];
+    }
   }
   if (sh_bad) {                                         // what was taken out of the tiles, to the rows that see it
 #pragma unroll 1
