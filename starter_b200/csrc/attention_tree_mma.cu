@@ -9,6 +9,12 @@
 // Places behind the sequence or in front of what a window leaves are copied as zeros, so whatever lies there adds nothing.  A value
 // that is no number must reach the rows that see it and no others, though a weight of zero times it is none: on pages that some row
 // does not see whole such entries are taken out of the tile, and put onto the results of the rows that see them at the end.
+//
+// What bounds it, with few rows, is the chain of dependent steps: 5 nodes of one sequence behind 1,500 tokens (32 heads of 128 on 8: 128 blocks of
+// three pages) take 8.3 us, where their 6 MB are worth 1: 1.3 us to the first copy (the step's arrays, the table), 1.3 until the page is there, 0.5 a page, 0.9
+// for the meeting of the warps, 1.8 for that of the blocks.  A second kernel for the meeting of more parts cost more than it gave (16,000 tokens, 16
+// rows: 29.6 us as 8 parts, 26.9 as 32 and a second kernel, but 2 more at 1,500); tiles of 64 rows were slower than two of 32 wherever tried.
+// With many rows it is mma.sync's issue: 128 pairs of 64 rows behind 1,500 tokens 41 us.
 #include "allow_smem.cuh"
 #include "attention_tree.cuh"
 

@@ -12,8 +12,9 @@
 // Every block walks its sequence's tree itself (a few shared-memory steps of a tree's depth; a launch of its own would cost more).  A thread then
 // moves one 16-byte column (4 bytes where rows do not allow it) of one entry's keys or values of one key/value head through all rows of the
 // way, eight rows on their way at a time: nodes come after their parents, so path[i] >= i grows with i, and what is written at row i has been
-// read, or is no row of the way.  What bounds it is the chain of the walk, the page numbers, a read and a write: 6 nodes of each of 16
-// sequences in 36 layers (23.6 MB) take 8 us, as blocks that moved 128-byte columns through shared memory one after another 49.
+// read, or is no row of the way.  What bounds it is the chain of the walk, the page numbers, a read and a write: 4 nodes of one sequence in 36
+// layers take 2.7 us, 6 nodes of each of 16 sequences (23.6 MB, worth 3.6 us) 4.6; as blocks that moved 128-byte columns through shared memory one
+// after another 49.
 #define CA_THREADS 256
 #define CA_MAX_NODES 256
 #define CA_FLIGHT 8
@@ -97,7 +98,8 @@ __global__ void __launch_bounds__(CA_THREADS) cache_accept_kernel(const AcceptAr
 // ------------------------------------------------------------------------------------------ pages
 //
 // Copies items (cache pages, a slot's state) of several tensors [outer, items, item_bytes]: item source[i] to item target[i], for every
-// outer index.  The pairs travel in the launch's own arguments, so nothing is uploaded.
+// outer index.  The pairs travel in the launch's own arguments, so nothing is uploaded.  A block copies one item, 16 bytes a thread at a time.
+// What bounds it is memory: 32 pages of 36 layers (604 MB read and written) take 104 us, 5.8 TB/s; one page of 8 layers 4.4 us, a launch.
 #define CP_MAX_TENSORS 16
 #define CP_MAX_PAIRS 256
 #define CP_THREADS 256

@@ -10,10 +10,11 @@
 // (an entry of another group has k entries in front of it).  Behind the pass the block finds those groups and reads them once more: a bar that k + 1
 // of them reach comes from the threads' best ones, what reaches it is ranked by counting, and so are the groups' entries.  A value and
 // an index make one 64-bit key, larger for what comes first, so that all keys differ.  (Candidates gathered in the pass itself, into a sorted
-// list a warp or a buffer a block, cost barriers and divergent code in every tile: 8 rows of 151,936 with 20 alternatives 30 and 17 us, 600
-// rows with 5 110 and 138.)  Entries that are no numbers have no key.
+// list a warp or a buffer a block, cost barriers and divergent code in every tile: 8 rows of 151,936 with 20 alternatives 30 and 17 us, 8.5 so; 600
+// rows with 5 110 and 138, 66 so.)  Entries that are no numbers have no key.
 //
-// A row is shared by the blocks of a cluster, whose results meet in the first one's hands.  What bounds it is reading the logits.
+// A row is shared by the blocks of a cluster, whose results meet in the first one's hands.  What bounds it is reading the logits where rows are many
+// (600 of 151,936 in float, 365 MB: 5.5 TB/s); of the 8.5 us of 8 rows the pass takes 2, the choice of the alternatives 3.5, the meeting 2.
 #include "allow_smem.cuh"
 #include "logprob_stats.cuh"
 
