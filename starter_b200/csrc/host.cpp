@@ -188,6 +188,59 @@ PyObject* fits(PyObject*, PyObject* const* args, Py_ssize_t n) {
   }
 }
 
+// Contiguous and on the current CUDA device.
+bool here(const at::Tensor& t) { return t.is_cuda() && t.layout() == at::kStrided && t.is_contiguous() && t.get_device() == c10::cuda::current_device(); }
+
+// items(t, dim): (address, how many in front of dimension `dim` (0 or 1), its size, bytes of one of its items) of a contiguous tensor on the current device,
+// None of any other.
+PyObject* items(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 2 || !THPVariable_Check(args[0])) Py_RETURN_NONE;
+  const long dim = PyLong_AsLong(args[1]);
+  if (dim == -1 && PyErr_Occurred()) return nullptr;
+  try {
+    const at::Tensor& t = THPVariable_Unpack(args[0]);
+    if (dim < 0 || dim > 1 || !here(t) || t.dim() <= dim) Py_RETURN_NONE;
+    const long long outer = dim ? t.size(0) : 1, count = t.size(dim);
+    return Py_BuildValue("LLLL", (long long)(intptr_t)t.data_ptr(), outer, count, t.numel() ? (long long)(t.numel() * t.element_size()) / (outer * count) : 0ll);
+  } catch (const std::exception&) {
+    Py_RETURN_NONE;
+  }
+}
+
+// page_rows(keys, values, page): (entries, pages, heads, bytes of a row of keys, of values) of a cache's storage [entries, pages, heads, page, dim], or of one
+// entry's without the first dimension, whose rows are words of four bytes, one or more of each; None of anything else.
+PyObject* page_rows(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 3 || !THPVariable_Check(args[0]) || !THPVariable_Check(args[1])) Py_RETURN_NONE;
+  const long page = PyLong_AsLong(args[2]);
+  if (page == -1 && PyErr_Occurred()) return nullptr;
+  try {
+    const at::Tensor &k = THPVariable_Unpack(args[0]), &v = THPVariable_Unpack(args[1]);
+    const int64_t d = k.dim();
+    if ((d != 4 && d != 5) || v.dim() != d || !here(k) || !here(v) || !k.numel() || !v.numel() || k.size(d - 2) != page) Py_RETURN_NONE;
+    for (int64_t i = 0; i < d - 1; ++i)
+      if (k.size(i) != v.size(i)) Py_RETURN_NONE;
+    const long long key_bytes = k.size(d - 1) * k.element_size(), value_bytes = v.size(d - 1) * v.element_size();
+    if ((key_bytes | value_bytes | (long long)(intptr_t)k.data_ptr() | (long long)(intptr_t)v.data_ptr()) & 3) Py_RETURN_NONE;
+    return Py_BuildValue("LLLLL", d == 5 ? (long long)k.size(0) : 1ll, (long long)k.size(d - 4), (long long)k.size(d - 3), key_bytes, value_bytes);
+  } catch (const std::exception&) {
+    Py_RETURN_NONE;
+  }
+}
+
+// A tuple of integers as sizes; false where it is not that.
+bool sizes_of(PyObject* o, int64_t* sizes) {
+  bool plain = true;
+  for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(o) && plain; ++i) {
+    plain = PyLong_Check(PyTuple_GET_ITEM(o, i));
+    if (plain) sizes[i] = PyLong_AsLongLong(PyTuple_GET_ITEM(o, i));
+  }
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    return false;
+  }
+  return plain;
+}
+
 // empty(like, shape, dtype=None): like.new_empty(shape, dtype=dtype).
 PyObject* empty(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if ((n == 2 || n == 3) && THPVariable_Check(args[0]) && PyTuple_Check(args[1]) && PyTuple_GET_SIZE(args[1]) <= 6) {
@@ -195,19 +248,11 @@ PyObject* empty(PyObject*, PyObject* const* args, Py_ssize_t n) {
       const at::Tensor& like = THPVariable_Unpack(args[0]);
       if (like.is_cuda() && !at::globalContext().deterministicAlgorithms() && (n == 2 || args[2] == Py_None || THPDtype_Check(args[2]))) {
         int64_t sizes[6];
-        const Py_ssize_t dims = PyTuple_GET_SIZE(args[1]);
-        bool plain = true;
-        for (Py_ssize_t i = 0; i < dims && plain; ++i) {
-          PyObject* o = PyTuple_GET_ITEM(args[1], i);
-          plain = PyLong_Check(o);
-          if (plain) sizes[i] = PyLong_AsLongLong(o);
-        }
-        if (plain && !PyErr_Occurred()) {
+        if (sizes_of(args[1], sizes)) {
           const at::ScalarType type =
               n == 2 || args[2] == Py_None ? like.scalar_type() : reinterpret_cast<THPDtype*>(args[2])->scalar_type;
-          return THPVariable_Wrap(at::Tensor(at::detail::empty_cuda(at::IntArrayRef(sizes, dims), type, like.device(), std::nullopt)));
+          return THPVariable_Wrap(at::Tensor(at::detail::empty_cuda(at::IntArrayRef(sizes, PyTuple_GET_SIZE(args[1])), type, like.device(), std::nullopt)));
         }
-        PyErr_Clear();
       }
     } catch (const std::exception&) {
     }
@@ -221,6 +266,63 @@ PyObject* empty(PyObject*, PyObject* const* args, Py_ssize_t n) {
   PyObject* out = PyObject_Vectorcall(made, call, 1, kw);
   Py_XDECREF(kw);
   Py_DECREF(made);
+  return out;
+}
+
+// empties(like, shape, shape, ...): small results of like's type, together in one allocation (each on a boundary of 16 bytes), or one by one.
+PyObject* empties(PyObject* self, PyObject* const* args, Py_ssize_t n) {
+  if (n < 2 || n > 9 || !THPVariable_Check(args[0])) {
+    PyErr_SetString(PyExc_TypeError, "empties(like, shape, ...) of up to eight shapes");
+    return nullptr;
+  }
+  PyObject* out = PyTuple_New(n - 1);
+  if (!out) return nullptr;
+  const at::Tensor& like = THPVariable_Unpack(args[0]);
+  if (like.is_cuda() && !at::globalContext().deterministicAlgorithms()) {
+    try {
+      int64_t sizes[8][6], first[8], total = 0;
+      bool plain = true;
+      for (Py_ssize_t i = 0; i + 1 < n && plain; ++i) {
+        plain = PyTuple_Check(args[i + 1]) && PyTuple_GET_SIZE(args[i + 1]) <= 6 && sizes_of(args[i + 1], sizes[i]);
+        int64_t count = 1;
+        for (Py_ssize_t d = 0; plain && d < PyTuple_GET_SIZE(args[i + 1]); ++d) {
+          plain = sizes[i][d] >= 0 && (sizes[i][d] == 0 || count <= (int64_t(1) << 40) / sizes[i][d]);
+          count *= plain ? sizes[i][d] : 0;
+        }
+        first[i] = total;
+        total += (count + 15) / 16 * 16;
+      }
+      if (plain) {
+        const at::Tensor all = at::detail::empty_cuda(at::IntArrayRef(&total, 1), like.scalar_type(), like.device(), std::nullopt);
+        for (Py_ssize_t i = 0; i + 1 < n; ++i) {
+          at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), all.dtype());
+          t.unsafeGetTensorImpl()->set_storage_offset(first[i]);
+          t.unsafeGetTensorImpl()->set_sizes_contiguous(at::IntArrayRef(sizes[i], PyTuple_GET_SIZE(args[i + 1])));
+          PyObject* wrapped = THPVariable_Wrap(std::move(t));
+          if (!wrapped) {
+            Py_DECREF(out);
+            return nullptr;
+          }
+          PyTuple_SET_ITEM(out, i, wrapped);
+        }
+        return out;
+      }
+    } catch (const std::exception&) {
+      for (Py_ssize_t i = 0; i + 1 < n; ++i) {
+        Py_XDECREF(PyTuple_GET_ITEM(out, i));
+        PyTuple_SET_ITEM(out, i, nullptr);
+      }
+    }
+  }
+  for (Py_ssize_t i = 0; i + 1 < n; ++i) {
+    PyObject* one[2] = {args[0], args[i + 1]};
+    PyObject* made = empty(self, one, 2);
+    if (!made) {
+      Py_DECREF(out);
+      return nullptr;
+    }
+    PyTuple_SET_ITEM(out, i, made);
+  }
   return out;
 }
 
@@ -366,7 +468,10 @@ PyObject* refuse_with(PyObject*, PyObject* function) {
 PyMethodDef methods[] = {
     {"need", (PyCFunction)(void (*)(void))need, METH_FASTCALL, nullptr},
     {"fits", (PyCFunction)(void (*)(void))fits, METH_FASTCALL, nullptr},
+    {"items", (PyCFunction)(void (*)(void))items, METH_FASTCALL, nullptr},
+    {"page_rows", (PyCFunction)(void (*)(void))page_rows, METH_FASTCALL, nullptr},
     {"empty", (PyCFunction)(void (*)(void))empty, METH_FASTCALL, nullptr},
+    {"empties", (PyCFunction)(void (*)(void))empties, METH_FASTCALL, nullptr},
     {"product", (PyCFunction)(void (*)(void))product, METH_FASTCALL, nullptr},
     {"block_steps", (PyCFunction)(void (*)(void))block_steps, METH_FASTCALL, nullptr},
     {"mixed_splits", (PyCFunction)(void (*)(void))mixed_splits, METH_FASTCALL, nullptr},

@@ -94,11 +94,12 @@ def _refuse(t, name, dtype=None, ndim=None):
 # launch, are native too (csrc/host.cpp).  The first call of any of them loads the native part and puts it in these names.
 
 def _bind():
-    global _need, _fits, _empty, _stream, _product, _block_steps, _mixed_splits
+    global _need, _fits, _empty, _empties, _items, _page_rows, _stream, _product, _block_steps, _mixed_splits
     host = build.load_host()
     host.refuse_with(_refuse)
     _need, _fits, _empty, _stream, _product = host.need, host.fits, host.empty, host.stream, host.product
     _block_steps, _mixed_splits = host.block_steps, host.mixed_splits
+    _empties, _items, _page_rows = host.empties, host.items, host.page_rows
     return host
 
 
@@ -116,6 +117,21 @@ def _fits(t, dtype, *sizes):
 
 def _empty(like, shape, dtype=None):
     return _bind().empty(like, shape, dtype)
+
+
+def _empties(like, *shapes):
+    """Small results of one call, in one allocation."""
+    return _bind().empties(like, *shapes)
+
+
+def _items(t, dim):
+    """``(address, outer, items, bytes an item)`` of a contiguous tensor on the current CUDA device, by the dimension that counts items; None of any other."""
+    return _bind().items(t, dim)
+
+
+def _page_rows(keys, values, page):
+    """``(entries, pages, heads, bytes of a row of keys, of values)`` of a cache's storage; None of anything else."""
+    return _bind().page_rows(keys, values, page)
 
 
 def _stream():
@@ -1542,32 +1558,30 @@ def cache_accept(stores, block_table, seq_slot, seq_q_start, seq_q_len, seq_kv_l
                 raise KernelError(f"{name} has {t.shape[0]} entries for {tokens.shape[0]} nodes")
     geometry = []
     for keys, values in stores:
-        shape = getattr(keys, "shape", ())
-        if len(shape) == 4:
-            shape = (1, *shape)
-            keys, values = (t[None] if isinstance(t, torch.Tensor) else t for t in (keys, values))
-        if len(shape) != 5 or not (_fits(keys, None, *shape[:3], PAGE_TOKENS, None) and _fits(values, None, *shape[:3], PAGE_TOKENS, None)):
-            for t in (keys, values):
-                _need(t, "cache pages")
-                _here(t, "cache pages")
-            raise KernelError(f"cache pages have shapes {tuple(keys.shape)} and {tuple(values.shape)}")
-        rows = shape[4] * keys.element_size(), values.shape[4] * values.element_size()
-        if not (rows[0] and rows[1] and shape[0] and shape[1] and shape[2]) or (rows[0] | rows[1] | keys.data_ptr() | values.data_ptr()) & 3:
-            raise KernelError(f"cache pages have shapes {tuple(keys.shape)} and {tuple(values.shape)}, rows of {rows[0]} and {rows[1]} bytes: the kernel "
-                              "moves words of four, one or more of each")
-        geometry.append((keys, values, rows, shape))
+        found = _page_rows(keys, values, PAGE_TOKENS)
+        if found is None:
+            _refuse_page_rows(keys, values)
+        geometry.append((keys, values, found))
     if not geometry:
         raise KernelError("no cache pages are given")
-    outs = _empty(tokens, (seqs,)), _empty(tokens, (seqs, max_q_len)), _empty(tokens, (seqs, max_q_len))
+    outs = to = _empties(tokens, (seqs,), (seqs, max_q_len), (seqs, max_q_len))
     if seqs:
-        lib = _lib("cache_pages")
-        for n, (keys, values, rows, (entries, pages, kv_heads, *_)) in enumerate(geometry):
-            count_to, path_to, taken_to = outs if n == 0 else (None, None, None)
-            rc = lib.sb_cache_accept(keys, values, rows[0], rows[1], entries, pages, kv_heads, block_table, block_table.shape[1], seq_slot,
-                                     seq_q_start, seq_q_len, seq_kv_len, seqs, tokens, parents, drawn, count_to, path_to, taken_to,
-                                     max_q_len, _stream())
+        lib, stride, stream = _lib("cache_pages"), block_table.shape[1], _stream()
+        for keys, values, (entries, pages, kv_heads, key_bytes, value_bytes) in geometry:
+            rc = lib.sb_cache_accept(keys, values, key_bytes, value_bytes, entries, pages, kv_heads, block_table, stride, seq_slot, seq_q_start,
+                                     seq_q_len, seq_kv_len, seqs, tokens, parents, drawn, *to, max_q_len, stream)
             _check(rc, "cache_accept")
+            to = None, None, None
     return outs
+
+
+def _refuse_page_rows(keys, values):
+    """What is wrong with a pair of ``cache_accept``'s stores."""
+    for t in (keys, values):
+        _need(t, "cache pages")
+        _here(t, "cache pages")
+    raise KernelError(f"cache pages have shapes {tuple(keys.shape)} and {tuple(values.shape)} of {keys.dtype} and {values.dtype}: the kernel moves rows of "
+                      f"[entries, pages, heads, {PAGE_TOKENS}, dim] by words of four bytes, one or more of each")
 
 
 # ---------------------------------------------------------------------------------------- pages
@@ -1598,16 +1612,15 @@ def cache_copy_pages(stores, source, target, dim=1):
     low, high = (min(pairs), max(pairs)) if n else (0, -1)
     described = array.array("q")
     for t in stores:
-        shape = t.shape if isinstance(t, torch.Tensor) else ()
-        if not _fits(t, None, *(None for _ in shape)) or len(shape) <= dim:
+        found = _items(t, dim)
+        if found is None:
             _need(t, "cache pages")
             _here(t, "cache pages")
-            raise KernelError(f"cache pages have shape {tuple(shape)}")
-        outer, items, size = shape[0] if dim else 1, shape[dim], t.numel() * t.element_size()
-        if low < 0 or high >= items:
-            raise KernelError(f"a page outside the {items} of the cache")
-        if size:                                 # (a latent's cache keeps no values)
-            described.extend((t.data_ptr(), outer, items, size // (outer * items)))
+            raise KernelError(f"cache pages have shape {tuple(t.shape)}")
+        if low < 0 or high >= found[2]:
+            raise KernelError(f"a page outside the {found[2]} of the cache")
+        if found[3]:                             # (a latent's cache keeps no values)
+            described.extend(found)
     if not n or not described:
         return
     entry, stream = _lib("cache_pages").sb_cache_copy, _stream()
