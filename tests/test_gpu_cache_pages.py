@@ -136,6 +136,23 @@ def test_accept_captured_and_replayed():
     assert count.tolist() == [len(w) for w in s.ways()]
 
 
+def test_accepted_rows_past_two_to_the_31_entries():
+    """Pages and entries of a store whose offsets pass 2^31 entries."""
+    s = Step([20, 9], [100, 30], entries=2, kv_heads=8, dims=(128, 128), vocab=2, seed=8)
+    shift = 2 ** 30 // (8 * PAGE * 128) + 5
+    wide = [torch.empty((2, shift + s.pages, 8, PAGE, 128), dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    for w, t in zip(wide, (s.keys, s.values)):
+        w[:, shift:] = t.cuda()
+    flat = lambda lists: ints([x for part in lists for x in part])  # noqa: E731
+    ops.cache_accept([tuple(wide)], torch.from_numpy(s.table).cuda() + shift, ints(s.slots), ints(s.starts[:-1]), ints(s.nodes),
+                     ints([p + n for p, n in zip(s.past, s.nodes)]), flat(s.tokens), flat(s.parents), flat(s.drawn), max_q_len=20)
+    for w, t in zip(wide, (s.keys, s.values)):
+        assert torch.equal(w[:, shift:].cpu(), s.moved(t))
+    before = wide[0][:, shift + 1].clone()
+    ops.cache_copy_pages([wide[0]], [shift + 1], [shift])
+    assert torch.equal(wide[0][:, shift], before) and torch.equal(wide[0][:, shift + 1], before)
+
+
 def test_accept_refusals():
     s = Step([8], [50])
     k, v = s.keys.cuda(), s.values.cuda()

@@ -201,6 +201,20 @@ def test_captured_and_replayed_on_a_stream(rows):
     assert torch.equal(out[3], w[3])
 
 
+def test_rows_past_two_to_the_31_entries():
+    """The last rows of 8.6 GB of logits."""
+    rows = 2 ** 31 // 150001 + 3
+    wide = torch.empty((rows, 150001), device="cuda")
+    x, t = logits(2, 150001, 9)
+    wide[:-2] = 0
+    wide[-2:] = x
+    got = ops.token_logprobs(wide, torch.cat([torch.zeros(rows - 2, dtype=torch.int32, device="cuda"), t]), top=4)
+    want = expected(x, t, 4)
+    near(got[0][-2:], want[0], want[4])
+    near(got[1][-2:], want[1], want[5])
+    assert torch.equal(got[3][-2:], want[3])
+
+
 def test_logprob_refusals():
     x, t = logits(4, 100)
     for args, kw in (((x.half(), t), {}), ((x, t.long()), {}), ((x, t[:-1]), {}), ((x.t(), t), {}), ((x[0], t), {}), ((x[:, :0], t), {}),

@@ -296,6 +296,20 @@ def test_keys_in_parts_on_the_plain_kernel(dtype, dim, parts):
     check(c, ops.attention_tree(**c.on_device(), kernel="plain", parts=parts))
 
 
+@pytest.mark.parametrize("kernel", ["plain", "mma", "tcgen05"])
+def test_pages_past_two_to_the_31_entries(kernel):
+    """The step's pages lie behind 2^31 entries of the stores (of each, 4.3 GB)."""
+    sees, depth = trees([20, 3], seed=4)
+    c = Case("bf16", 16, 8, 128, sees, [300, 70], depth, seed=4)
+    args, shift = c.on_device(), 2 ** 31 // (8 * PAGE * 128) + 3
+    for name in ("k_store", "v_store"):
+        wide = torch.empty((shift + c.pages, 8, PAGE, 128), dtype=torch.bfloat16, device="cuda")
+        wide[shift:] = args[name]
+        args[name] = wide
+    args["block_table"] = args["block_table"] + shift
+    check(c, ops.attention_tree(**args, kernel=kernel))
+
+
 @pytest.mark.parametrize("parts", [1, 2])
 def test_a_wait_of_the_tree_attention_that_runs_out_is_reported(parts):
     """Half of a step's values are not copied: the wait gives up, the status says so, and the next call is right."""
