@@ -7,7 +7,7 @@
 // references, sums and outputs of their own, which meet at the end.  Everything is float; a result is rounded to the working type
 // once.  Up to eight parts of a sequence's keys are the blocks of one cluster and meet in shared memory.
 //
-// What bounds it: 2 sequences of 13 nodes of 16 heads behind 300 tokens, 256 blocks of two tiles, take 15.8 us: 5 until the first tile is there (the
+// What bounds it: 2 sequences of 13 nodes of 16 heads behind 300 tokens, 256 blocks of two tiles, take 15.4 us: 5 until the first tile is there (the
 // step's arrays, the page's number, the page, which the four blocks of a head's rows all read), 2.9 a tile (the products of queries and
 // keys 1.2, of weights and values 1.1, most of it the shared memory's rate), 3.5 for the meeting of the blocks.  Keys a lane each and
 // rows a warp each read the tile four times over: 17.2; copies and products in turn and a second kernel for the meeting: 33.0.
@@ -80,7 +80,6 @@ __global__ void __launch_bounds__(TP_THREADS, NJ == 1 ? 3 : 1) attention_tree_pl
   __shared__ int firsts[TP_TILE];                     // the rows' windows' first places
   __shared__ float sh_m[TP_WARPS][TP_TILE], sh_l[TP_WARPS][TP_TILE];
   __shared__ float cl_m[TP_TILE], cl_l[TP_TILE];      // the rows' references and sums
-  __shared__ int sh_low;
   pdl_trigger();
   pdl_wait();
   const int split = blockIdx.z, seq = blockIdx.y / a.kv_heads, kvh = blockIdx.y - seq * a.kv_heads;
@@ -92,18 +91,8 @@ __global__ void __launch_bounds__(TP_THREADS, NJ == 1 ? 3 : 1) attention_tree_pl
   const int* pages = a.block_table + (size_t)a.seq_slot[seq] * a.table_stride;
   const T* q = (const T*)a.q;
 
-  if (a.window > 0) {
-    if (tid == 0) sh_low = past;
-    __syncthreads();
-    if (tid < TP_TILE) {
-      const int first = a.tok_pos[start + min(row0 + tid, n_rows - 1) / group] - a.window + 1;
-      firsts[tid] = first;
-      atomicMin(&sh_low, max(first, 0));
-    }
-    __syncthreads();
-  }
   // tiles of half a page, from the one with the first place any row sees
-  const int tile_lo = (a.window > 0 ? sh_low : 0) / TP_KEYS, tiles = (kv_len + TP_KEYS - 1) / TP_KEYS - tile_lo;
+  const int tile_lo = tree_low(a, past) / TP_KEYS, tiles = (kv_len + TP_KEYS - 1) / TP_KEYS - tile_lo;
   const int per = (tiles + a.splits - 1) / a.splits;
   const int begin = tile_lo + min(split * per, tiles), n_tiles = tile_lo + min((split + 1) * per, tiles) - begin;
 
@@ -133,8 +122,8 @@ __global__ void __launch_bounds__(TP_THREADS, NJ == 1 ? 3 : 1) attention_tree_pl
 
   // the rows' masks, a word a thread, and queries (rows behind the last look like the last)
   static_assert(TP_TILE * TREE_MAX_WORDS == TP_THREADS, "a word of the masks for every thread");
-  const uint32_t word = tree_mask_word(a, start, min(row0 + tid / TREE_MAX_WORDS, n_rows - 1) / group, tid % TREE_MAX_WORDS, q_len,
-                                       a.window > 0 ? firsts[tid / TREE_MAX_WORDS] : 0);
+  const int my_node = min(row0 + tid / TREE_MAX_WORDS, n_rows - 1) / group, my_first = a.window > 0 ? a.tok_pos[start + my_node] - a.window + 1 : 0;
+  const uint32_t word = tree_mask_word(a, start, my_node, tid % TREE_MAX_WORDS, q_len, my_first, past);
 #pragma unroll
   for (int n = 0; n < TP_TILE / TP_WARPS; ++n) {
     const int r = warp + n * TP_WARPS, row = min(row0 + r, n_rows - 1);
@@ -153,6 +142,7 @@ __global__ void __launch_bounds__(TP_THREADS, NJ == 1 ? 3 : 1) attention_tree_pl
     }
   }
   masks[tid / TREE_MAX_WORDS][tid % TREE_MAX_WORDS] = word;
+  if (tid % TREE_MAX_WORDS == 0) firsts[tid / TREE_MAX_WORDS] = my_first;
 
   // A lane's key of a tile and its rows: group, group + 4, ...
   const int key = warp * TP_WARP_KEYS + (lane & 7), row_of = lane >> 3;
@@ -194,7 +184,7 @@ __global__ void __launch_bounds__(TP_THREADS, NJ == 1 ? 3 : 1) attention_tree_pl
     bool moved = false;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int r = row_of + 4 * i, first = a.window > 0 ? firsts[r] : 0;
+      const int r = row_of + 4 * i, first = firsts[r];
       s[i] += t[i];
       if (j0 + TP_KEYS > past || j0 < first) {        // (what is cached and inside the window is seen)
         const uint32_t view = (uint32_t)tree_view(masks[r], first, past, kv_len, j0);

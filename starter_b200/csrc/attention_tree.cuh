@@ -1,7 +1,7 @@
 // What the kernels of tree attention share: the step's arrays, a packed row's node and head, and what a node may look at.
 //
 // A step brings, per sequence, `q_len` nodes of a drafted tree behind `past = kv_len - q_len` cached tokens.  Node i's key and value
-// are filed at place past + i of the sequence, whatever its position; its position (tok_pos, past + its depth) is what its
+// are filed at place past + i of the sequence, whatever its position; its position (tok_pos, past + its depth, below kv_len) is what its
 // rotation and a window go by.  With mask_i the bits of the nodes that node i looks at (itself and those above it, or what the caller
 // likes):
 //     o_i = sum_j p_ij v_j / sum_j p_ij,   p_ij = exp(scale q_i k_j),
@@ -64,10 +64,14 @@ __device__ __forceinline__ uint64_t tree_view(const uint32_t* bits, int first, i
   if (hidden > 0) view &= hidden < 64 ? ~0ull << hidden : 0ull;      // cached places in front of the window
   return view;
 }
-// Word w of the mask of a sequence's node, without the nodes in front of its window (first: its first place).
-__device__ __forceinline__ uint32_t tree_mask_word(const TreeArgs& a, int start, int node, int w, int q_len, int first) {
+// The first place any node sees and the one from which on every node sees all that is cached, as far as the lengths say: positions lie between the first
+// behind what is cached and the sequence's last, so nothing has to be read for them.
+__device__ __forceinline__ int tree_low(const TreeArgs& a, int past) { return a.window > 0 ? max(past - a.window + 1, 0) : 0; }
+__device__ __forceinline__ int tree_high(const TreeArgs& a, int past, int kv_len) { return a.window > 0 ? min(max(kv_len - a.window, 0), past) : 0; }
+// Word w of the mask of a sequence's node, without the nodes in front of its window (first: its first place; up to `past` it leaves out none).
+__device__ __forceinline__ uint32_t tree_mask_word(const TreeArgs& a, int start, int node, int w, int q_len, int first, int past) {
   uint32_t bits = w < a.words ? a.mask[(size_t)(start + node) * a.words + w] : 0u;
-  if (a.window > 0) {
+  if (a.window > 0 && first > past) {
     for (uint32_t left = bits; left; left &= left - 1) {
       const int m = 32 * w + __ffs(left) - 1;
       if (m >= q_len || a.tok_pos[start + m] < first) bits &= ~(left & -left);

@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(TM_THREADS) attention_tree_mma_kernel(const Tr
   __shared__ int sh_first[ROWS];                        // their windows' first places
   __shared__ float sh_m[WK][ROWS], sh_l[WK][ROWS];
   __shared__ float2 cl_ml[ROWS];                        // the block's reference and sum of a row
-  __shared__ int sh_low, sh_high, sh_bad;
+  __shared__ int sh_bad;
 
   pdl_trigger();
   pdl_wait();
@@ -102,19 +102,8 @@ __global__ void __launch_bounds__(TM_THREADS) attention_tree_mma_kernel(const Tr
   const int* pages = a.block_table + (size_t)a.seq_slot[seq] * a.table_stride;
   const int node0 = row0 / group, n_nodes = (min(row0 + ROWS, n_rows) - 1) / group - node0 + 1;
 
-  if (a.window > 0) {
-    if (tid == 0) { sh_low = past; sh_high = 0; }
-    __syncthreads();
-    for (int n = tid; n < n_nodes; n += TM_THREADS) {
-      const int first = a.tok_pos[start + node0 + n] - a.window + 1;
-      sh_first[n] = first;
-      atomicMin(&sh_low, max(first, 0));                // the first place any row sees
-      atomicMax(&sh_high, min(first, past));            // from here on every row sees all that is cached
-    }
-    __syncthreads();
-  }
   if (tid == 0) sh_bad = 0;
-  const int low = a.window > 0 ? sh_low : 0, high = a.window > 0 ? sh_high : 0;
+  const int low = tree_low(a, past), high = tree_high(a, past, kv_len);
   const int first_page = low / SB_PAGE_TOKENS, end_page = (kv_len + SB_PAGE_TOKENS - 1) / SB_PAGE_TOKENS;
   const int per_split = (end_page - first_page + a.splits - 1) / a.splits;
   const int p_begin = first_page + split * per_split, n_pages = max(min(p_begin + per_split, end_page) - p_begin, 0);
@@ -135,7 +124,16 @@ __global__ void __launch_bounds__(TM_THREADS) attention_tree_mma_kernel(const Tr
 #pragma unroll
   for (int i = 0; i < TM_STAGES - 1; ++i) load_page(i);
 
-  // ---- while those are on their way: the tile's queries (rows behind the last are zero) and its nodes' masks
+  // ---- while those are on their way: the tile's nodes' masks and queries (rows behind the last are zero)
+  constexpr int WORDS = ROWS * TREE_MAX_WORDS / TM_THREADS;
+  uint32_t words[WORDS];
+  int firsts[WORDS];
+#pragma unroll
+  for (int i = 0; i < WORDS; ++i) {
+    const int n = min((tid + i * TM_THREADS) / TREE_MAX_WORDS, n_nodes - 1);
+    firsts[i] = a.window > 0 ? a.tok_pos[start + node0 + n] - a.window + 1 : 0;
+    words[i] = tree_mask_word(a, start, node0 + n, tid % TREE_MAX_WORDS, q_len, firsts[i], past);
+  }
 #pragma unroll
   for (int idx0 = 0; idx0 < ROWS * C; idx0 += TM_THREADS) {
     const int idx = idx0 + tid, r = idx / C, c = idx % C, row = row0 + r;
@@ -145,9 +143,11 @@ __global__ void __launch_bounds__(TM_THREADS) attention_tree_mma_kernel(const Tr
       v = *reinterpret_cast<const uint4*>((const bf16*)a.q + ((size_t)(start + row / group) * a.heads + kvh * group + row % group) * D + c * 8);
     *reinterpret_cast<uint4*>(q_tile + tile_offset<D>(r, c)) = v;
   }
-  for (int idx = tid; idx < n_nodes * TREE_MAX_WORDS; idx += TM_THREADS) {
-    const int n = idx / TREE_MAX_WORDS, w = idx % TREE_MAX_WORDS;
-    sh_mask[n][w] = tree_mask_word(a, start, node0 + n, w, q_len, a.window > 0 ? sh_first[n] : 0);
+#pragma unroll
+  for (int i = 0; i < WORDS; ++i) {
+    const int n = (tid + i * TM_THREADS) / TREE_MAX_WORDS;
+    sh_mask[n][tid % TREE_MAX_WORDS] = words[i];
+    if (tid % TREE_MAX_WORDS == 0) sh_first[n] = firsts[i];
   }
   __syncthreads();
 
@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(TM_THREADS) attention_tree_mma_kernel(const Tr
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     node[h] = min(row0 + wr * 16 + (lane >> 2) + 8 * h, n_rows - 1) / group - node0;
-    from[h] = a.window > 0 ? sh_first[node[h]] : 0;
+    from[h] = sh_first[node[h]];
   }
   float o[NBLK][4];
 #pragma unroll
@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(TM_THREADS) attention_tree_mma_kernel(const Tr
       const int r = idx / (D / 2), d = (idx - r * (D / 2)) * 2, n = (row0 + r) / group - node0;
       float2* x = reinterpret_cast<float2*>(sh_o + (size_t)r * DP + d);
       for (int j = p_begin * SB_PAGE_TOKENS; j < min((p_begin + n_pages) * SB_PAGE_TOKENS, kv_len); ++j) {
-        if (!(tree_view(sh_mask[n], a.window > 0 ? sh_first[n] : 0, past, kv_len, j) & 1ull)) continue;
+        if (!(tree_view(sh_mask[n], sh_first[n], past, kv_len, j) & 1ull)) continue;
         const uint32_t v = *reinterpret_cast<const uint32_t*>((const bf16*)a.v_store + page_row(pages[j / SB_PAGE_TOKENS], kvh, j % SB_PAGE_TOKENS, a.kv_heads, D) + d);
         if (no_number(v)) x->x += __uint_as_float(v << 16);
         if (no_number(v >> 16)) x->y += __uint_as_float(v & 0xffff0000u);

@@ -7,7 +7,7 @@
 // with S and O of both tiles in tensor memory.  Warps 0-3 and 4-7 are the softmax of tile 0 and 1 (thread = row = tensor-memory lane), warp 8
 // brings keys and values by TMA, warps 9 and 10 issue the products of tile 0 and 1: the schedule of the prompt attention
 // (attention_prefill_tc.cu), with all rows of a sequence's tree on one copy of its keys.  The queries of a tile lie in up to 128 pieces of
-// the packed rows; every softmax thread puts its own row into shared memory.
+// the packed rows; a softmax warp puts its own rows into shared memory.
 //
 // A row's view of a page is 64 bits: ones for what is cached (from its window's first place on), then the bits of its mask, shifted to where
 // the nodes begin in the page.  Only pages that some row does not see whole are masked.  On those a value that is no number is taken out of
@@ -18,7 +18,7 @@
 //
 // What bounds it is the softmax: a step of 128 keys takes 1.07 us with one tile and 1.5 with two, of which the exponentials of 2 x 128 x 128
 // scores are worth 1.07 at 16 a clock and the products 0.55.  16 sequences of 64 nodes behind up to 4,096 tokens each (32 heads of 128 on
-// 8, 128 blocks) take 69 us, 207 MB and 41 GFLOP that are worth 31: the longest sequence's 33 steps, 50 us, behind which the other SMs rest.  Tried
+// 8, 128 blocks) take 67 us, 207 MB and 41 GFLOP that are worth 31: the longest sequence's 33 steps, 50 us, behind which the other SMs rest.  Tried
 // and slower: a cubic in place of every fourth exponential (1.54 us a step) or every second (1.80); sixteen softmax warps, two threads a row (1.78: the
 // weights no longer fit in registers in front of the wait for the product before); both tiles on the same 128 rows where there are no more, every
 // second step each (16 x 32 nodes 57.7 us against 49.7: a copy's way from memory lies in every step).
@@ -94,7 +94,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
   uint8_t* ring = p_sm + 2 * P_BYTES;                     // three buffers, in the order of use: K0 K1 V0 K2 V1 K3 V2 ...
   __shared__ uint64_t q_ready[2], full[3], empty[3], s_ready[2], s_free[2], p_ready[2], o_ready[2], apart;
   __shared__ uint32_t tmem_holder;
-  __shared__ int abort_flag, sh_low, sh_high, sh_bad;
+  __shared__ int abort_flag, sh_bad;
   float2 row_state = make_float2(-INFINITY, 0.f);         // keys in parts: a row's reference and sum
 
   pdl_trigger();
@@ -105,7 +105,6 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
   const int group = a.heads / a.kv_heads, row0 = block * TT_ROWS, n_rows = q_len * group;
   if (row0 >= n_rows) return;                             // (the same in every block of a cluster)
   const int rows_valid = min(TT_ROWS, n_rows - row0), tiles = rows_valid > TC_BQ ? 2 : 1;
-  const int node0 = row0 / group, n_nodes = (row0 + rows_valid - 1) / group - node0 + 1;
   const int* pages = a.block_table + (size_t)a.seq_slot[seq] * a.table_stride;
   // the warp's number as a value the compiler knows to be the same in every lane
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -121,8 +120,6 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
     }
     mbar_init(&apart, 1);
     abort_flag = 0;
-    sh_low = a.window > 0 ? past : 0;
-    sh_high = 0;
     sh_bad = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -131,15 +128,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem_base = tmem_holder;
-  if (a.window > 0) {
-    for (int n = threadIdx.x; n < n_nodes; n += TT_THREADS) {
-      const int first = a.tok_pos[start + node0 + n] - a.window + 1;
-      atomicMin(&sh_low, max(first, 0));                  // the first place any row sees
-      atomicMax(&sh_high, min(first, past));              // from here on every row sees all that is cached
-    }
-    __syncthreads();
-  }
-  const int page_lo = sh_low / SB_PAGE_TOKENS, page_hi = (kv_len - 1) / SB_PAGE_TOKENS, high = sh_high;
+  const int page_lo = tree_low(a, past) / SB_PAGE_TOKENS, page_hi = (kv_len - 1) / SB_PAGE_TOKENS, high = tree_high(a, past, kv_len);
   int n_steps = (page_hi - page_lo) / 2 + 1, first_step = 0;
   if constexpr (PARTS) {                                  // this CTA's steps
     const int per = (n_steps + splits - 1) / splits;
@@ -243,31 +232,35 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
     // only when a row's maximum has outgrown the reference by more than 2^8, so most steps only produce P.
     const int t = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
     const int row = row0 + min(t * TC_BQ + r, rows_valid - 1), node = row / group;   // (rows behind the last look like the last)
-    const bool valid = t * TC_BQ + r < rows_valid;
     const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
     const uint32_t tmem_s = tmem_base + t * TT_BK + lane_addr, tmem_o = tmem_base + 2 * TT_BK + t * 128 + lane_addr;
     uint8_t* p_row = p_sm + t * P_BYTES + r * 128;
-    const size_t at = ((size_t)(start + node) * a.heads + kvh * group + row % group) * D;
+    const int at = (start + node) * a.heads + kvh * group + row % group;   // the row's place among all heads' rows
+    const int first = a.window > 0 ? a.tok_pos[start + node] - a.window + 1 : 0;
+    uint32_t bits[TREE_MAX_WORDS];
+#pragma unroll
+    for (int w = 0; w < TREE_MAX_WORDS; ++w) bits[w] = tree_mask_word(a, start, node, w, q_len, first, past);
+    // Queries and results come and go 16 bytes a lane, LANES lanes a row, through shared memory (a row a lane: 32 rows a request, 2 us of 69).
+    constexpr int LANES = 8 * DC;
+    const int piece = lane % LANES;
     {
       // K-major A operand: 64-element chunk dc, 16-byte column c ^ (r % 8) of row r
-      const uint4* src = reinterpret_cast<const uint4*>((const bf16*)a.q + at);
-      uint4 v[8];
+      uint8_t* q_tile = q_sm + t * Q_BYTES + (piece >> 3) * SUB;
+      uint4 v[LANES];
 #pragma unroll
-      for (int dc = 0; dc < DC; ++dc) {
+      for (int n = 0; n < LANES; ++n) {
+        const int from = __shfl_sync(0xffffffffu, at, n * (32 / LANES) + lane / LANES);
+        v[n] = *reinterpret_cast<const uint4*>((const bf16*)a.q + (size_t)from * D + piece * 8);
+      }
 #pragma unroll
-        for (int c = 0; c < 8; ++c) v[c] = src[dc * 8 + c];
-#pragma unroll
-        for (int c = 0; c < 8; ++c)
-          *reinterpret_cast<uint4*>(q_sm + t * Q_BYTES + dc * SUB + r * 128 + ((c ^ (r & 7)) << 4)) = v[c];
+      for (int n = 0; n < LANES; ++n) {
+        const int to = quarter * 32 + n * (32 / LANES) + lane / LANES;
+        *reinterpret_cast<uint4*>(q_tile + to * 128 + (((piece & 7) ^ (to & 7)) << 4)) = v[n];
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(&q_ready[t]);
     }
-    const int first = a.window > 0 ? a.tok_pos[start + node] - a.window + 1 : 0;
-    uint32_t bits[TREE_MAX_WORDS];
-#pragma unroll
-    for (int w = 0; w < TREE_MAX_WORDS; ++w) bits[w] = tree_mask_word(a, start, node, w, q_len, first);
     float m_ref = -INFINITY, l_run = 0.f;
     bool ok = true;
     // the whole warp goes on or the whole warp stops: tensor memory is read and written by warps
@@ -387,7 +380,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
       const bool bad = *(volatile int*)&sh_bad != 0;
       if constexpr (PARTS) row_state = make_float2(m_ref, l_run);
       const float inv = l_run > 0.f ? 1.f / l_run : l_run == 0.f ? 0.f : l_run;
-      bf16* dst = (bf16*)a.out + at;
+      uint8_t* o_row = p_sm + t * P_BYTES + r * (D * 2);   // the results pass through the weights' place
 #pragma unroll 1
       for (int c = 0; c < D; c += 32) {
         float ov[32];
@@ -409,7 +402,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
           for (int d = 0; d < 32; d += 4)
             *reinterpret_cast<float4*>(part_piece<64, D>(p_sm + t * P_BYTES, q_sm + t * Q_BYTES, r, (c + d) / 4)) =
                 make_float4(ov[d], ov[d + 1], ov[d + 2], ov[d + 3]);
-        } else if (valid) {
+        } else {
 #pragma unroll
           for (int d = 0; d < 32; d += 8) {
             uint32_t w[4];
@@ -418,8 +411,17 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
               const __nv_bfloat162 two = __floats2bfloat162_rn(ov[d + 2 * e] * inv, ov[d + 2 * e + 1] * inv);
               w[e] = *reinterpret_cast<const uint32_t*>(&two);
             }
-            *reinterpret_cast<uint4*>(dst + c + d) = make_uint4(w[0], w[1], w[2], w[3]);
+            *reinterpret_cast<uint4*>(o_row + ((((c + d) / 8) ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
           }
+        }
+      }
+      if constexpr (!PARTS) {
+        __syncwarp();
+#pragma unroll
+        for (int n = 0; n < LANES; ++n) {
+          const int from = n * (32 / LANES) + lane / LANES, to = __shfl_sync(0xffffffffu, at, from);
+          const uint4 v = *reinterpret_cast<const uint4*>(o_row + (from - lane) * (D * 2) + ((piece ^ (from & 7)) << 4));
+          if (t * TC_BQ + quarter * 32 + from < rows_valid) *reinterpret_cast<uint4*>((bf16*)a.out + (size_t)to * D + piece * 8) = v;
         }
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -433,39 +435,48 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
     __syncthreads();
     if (threadIdx.x < TT_ROWS) ml[threadIdx.x] = row_state;
     cluster_barrier();
-    // every CTA joins its share of the rows: 16 threads a row, D / 16 columns each
-    const int share = (rows_valid + splits - 1) / splits, c = (threadIdx.x & 15) * (D / 16);
+    // every CTA joins its share of the rows: D / 8 threads a row, 8 columns each
+    const int share = (rows_valid + splits - 1) / splits, c = threadIdx.x % (D / 8) * 8;
     if (threadIdx.x < TT_ROWS) {
-      for (int n = threadIdx.x >> 4; n < share; n += TT_ROWS / 16) {
+      for (int n = threadIdx.x / (D / 8); n < share; n += TT_ROWS / (D / 8)) {
         const int mine = part * share + n;
         if (mine >= rows_valid) break;
         const int t = mine / TC_BQ, r = mine % TC_BQ;
+        // (all loads in front of what they decide: a part without keys filed nothing, and what is read there is not used)
         float2 ps[TT_MAX_SPLITS];
-        float top = -INFINITY, sum = 0.f, o[D / 16];
+        float4 x[TT_MAX_SPLITS][2];
+        float top = -INFINITY, sum = 0.f, o[8];
 #pragma unroll
         for (int p = 0; p < TT_MAX_SPLITS; ++p) {
-          ps[p] = p < splits ? peer_load2(peer_u32(ml + mine, p)) : make_float2(-INFINITY, 0.f);
-          if (ps[p].y != 0.f) top = fmaxf(top, ps[p].x);
+          ps[p] = make_float2(-INFINITY, 0.f);
+          if (p >= splits) continue;
+          ps[p] = peer_load2(peer_u32(ml + mine, p));
+#pragma unroll
+          for (int d = 0; d < 2; ++d)
+            x[p][d] = peer_load4(peer_u32(part_piece<64, D>(p_sm + t * P_BYTES, q_sm + t * Q_BYTES, r, c / 4 + d), p));
         }
 #pragma unroll
-        for (int d = 0; d < D / 16; ++d) o[d] = 0.f;
+        for (int p = 0; p < TT_MAX_SPLITS; ++p)
+          if (ps[p].y != 0.f) top = fmaxf(top, ps[p].x);
+#pragma unroll
+        for (int d = 0; d < 8; ++d) o[d] = 0.f;
 #pragma unroll
         for (int p = 0; p < TT_MAX_SPLITS; ++p) {
-          // (a part without keys filed nothing; one whose sum is no number has a score that is none, which is the row's result)
+          // (a part whose sum is no number has a score that is none, which is the row's result)
           if (p >= splits || ps[p].y == 0.f) continue;
           const float w = fast_exp2(ps[p].x - top);
           sum = fmaf(w, ps[p].y, sum);
 #pragma unroll
-          for (int d = 0; d < D / 16; d += 4) {
-            const float4 x = peer_load4(peer_u32(part_piece<64, D>(p_sm + t * P_BYTES, q_sm + t * Q_BYTES, r, (c + d) / 4), p));
-            o[d] = fmaf(w, x.x, o[d]); o[d + 1] = fmaf(w, x.y, o[d + 1]); o[d + 2] = fmaf(w, x.z, o[d + 2]); o[d + 3] = fmaf(w, x.w, o[d + 3]);
+          for (int d = 0; d < 2; ++d) {
+            o[4 * d] = fmaf(w, x[p][d].x, o[4 * d]); o[4 * d + 1] = fmaf(w, x[p][d].y, o[4 * d + 1]);
+            o[4 * d + 2] = fmaf(w, x[p][d].z, o[4 * d + 2]); o[4 * d + 3] = fmaf(w, x[p][d].w, o[4 * d + 3]);
           }
         }
         const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
         const int row = row0 + mine;
         bf16* dst = (bf16*)a.out + ((size_t)(start + row / group) * a.heads + kvh * group + row % group) * D + c;
 #pragma unroll
-        for (int d = 0; d < D / 16; d += 4) {
+        for (int d = 0; d < 8; d += 4) {
           const __nv_bfloat162 two = __floats2bfloat162_rn(o[d] * inv, o[d + 1] * inv), more = __floats2bfloat162_rn(o[d + 2] * inv, o[d + 3] * inv);
           *reinterpret_cast<uint2*>(dst + d) = make_uint2(*reinterpret_cast<const uint32_t*>(&two), *reinterpret_cast<const uint32_t*>(&more));
         }

@@ -1451,7 +1451,7 @@ def attention_tree(q, k_store, v_store, block_table, seq_slot, seq_q_start, seq_
     ``q`` ``[T, heads * head_dim]`` packed by sequence; the ``seq_*`` arrays describe each sequence of the step as they do for
     ``attention_prefill``: its nodes are the rows ``seq_q_start`` to ``+ seq_q_len``, their keys and values are filed behind its
     ``seq_kv_len - seq_q_len`` cached tokens, node i's at place ``seq_kv_len - seq_q_len + i``.  ``tok_pos`` int32 ``[T]`` are the nodes'
-    positions (cached tokens plus depth).  Every node sees the cached tokens and, of its sequence's nodes, those whose bit is set in its
+    positions (cached tokens plus depth, so below ``seq_kv_len``).  Every node sees the cached tokens and, of its sequence's nodes, those whose bit is set in its
     row of ``tree_mask`` (int32 ``[T, words]``, node m is bit m % 32 of word m // 32); with ``window`` only what lies less than
     ``window`` positions before it.  A node that sees nothing gets zeros.  ``max_q_len``: the longest ``seq_q_len`` (at most
     ``TREE_MAX_NODES``; by default what the words hold); rows that belong to no sequence hold nothing.  ``kv_hint``: the longest
