@@ -14,7 +14,7 @@
 // three pages) take 8.3 us, where their 6 MB are worth 1: 1.3 us to the first copy (the step's arrays, the table), 1.3 until the page is there, 0.5 a page, 0.9
 // for the meeting of the warps, 1.8 for that of the blocks.  A second kernel for the meeting of more parts cost more than it gave (16,000 tokens, 16
 // rows: 29.6 us as 8 parts, 26.9 as 32 and a second kernel, but 2 more at 1,500); tiles of 64 rows were slower than two of 32 wherever tried.
-// With many rows it is mma.sync's issue: 128 pairs of 64 rows behind 1,500 tokens 41 us.
+// With many rows it is mma.sync's issue: 128 pairs of 64 rows behind 1,500 tokens 38 us.
 #include "allow_smem.cuh"
 #include "attention_tree.cuh"
 
@@ -78,7 +78,7 @@ template <int D> __device__ __forceinline__ int tile_offset(int row, int chunk) 
 __device__ __forceinline__ bool no_number(uint32_t half) { return (half & 0x7f80u) == 0x7f80u; }
 
 template <int D, int WR, bool CLUSTER>
-__global__ void __launch_bounds__(TM_THREADS) attention_tree_mma_kernel(const TreeArgs a) {
+__global__ void __launch_bounds__(TM_THREADS, D > 64 ? 2 : 4) attention_tree_mma_kernel(const TreeArgs a) {
   constexpr int C = D / 8, PAGE_BYTES = SB_PAGE_TOKENS * D * 2, STAGE_BYTES = 2 * PAGE_BYTES;
   constexpr int KSTEPS = D / 16, NBLK = D / 8;
   constexpr int WK = TM_WARPS / WR, KEYS = SB_PAGE_TOKENS / WK, KBLK = KEYS / 8, ROWS = 16 * WR;

@@ -236,13 +236,11 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
     const uint32_t tmem_s = tmem_base + t * TT_BK + lane_addr, tmem_o = tmem_base + 2 * TT_BK + t * 128 + lane_addr;
     uint8_t* p_row = p_sm + t * P_BYTES + r * 128;
     const int at = (start + node) * a.heads + kvh * group + row % group;   // the row's place among all heads' rows
-    const int first = a.window > 0 ? a.tok_pos[start + node] - a.window + 1 : 0;
-    uint32_t bits[TREE_MAX_WORDS];
-#pragma unroll
-    for (int w = 0; w < TREE_MAX_WORDS; ++w) bits[w] = tree_mask_word(a, start, node, w, q_len, first, past);
     // Queries and results come and go 16 bytes a lane, LANES lanes a row, through shared memory (a row a lane: 32 rows a request, 2 us of 69).
     constexpr int LANES = 8 * DC;
     const int piece = lane % LANES;
+    int first = 0;
+    uint32_t bits[TREE_MAX_WORDS];
     {
       // K-major A operand: 64-element chunk dc, 16-byte column c ^ (r % 8) of row r
       uint8_t* q_tile = q_sm + t * Q_BYTES + (piece >> 3) * SUB;
@@ -252,6 +250,9 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
         const int from = __shfl_sync(0xffffffffu, at, n * (32 / LANES) + lane / LANES);
         v[n] = *reinterpret_cast<const uint4*>((const bf16*)a.q + (size_t)from * D + piece * 8);
       }
+      if (a.window > 0) first = a.tok_pos[start + node] - a.window + 1;
+#pragma unroll
+      for (int w = 0; w < TREE_MAX_WORDS; ++w) bits[w] = tree_mask_word(a, start, node, w, q_len, first, past);
 #pragma unroll
       for (int n = 0; n < LANES; ++n) {
         const int to = quarter * 32 + n * (32 / LANES) + lane / LANES;
@@ -435,31 +436,32 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
     __syncthreads();
     if (threadIdx.x < TT_ROWS) ml[threadIdx.x] = row_state;
     cluster_barrier();
-    // every CTA joins its share of the rows: D / 8 threads a row, 8 columns each
-    const int share = (rows_valid + splits - 1) / splits, c = threadIdx.x % (D / 8) * 8;
+    // every CTA joins its share of the rows: 16 threads a row, D / 16 columns each
+    constexpr int COLS = D / 16;
+    const int share = (rows_valid + splits - 1) / splits, c = (threadIdx.x & 15) * COLS;
     if (threadIdx.x < TT_ROWS) {
-      for (int n = threadIdx.x / (D / 8); n < share; n += TT_ROWS / (D / 8)) {
+      for (int n = threadIdx.x >> 4; n < share; n += TT_ROWS / 16) {
         const int mine = part * share + n;
         if (mine >= rows_valid) break;
         const int t = mine / TC_BQ, r = mine % TC_BQ;
         // (all loads in front of what they decide: a part without keys filed nothing, and what is read there is not used)
         float2 ps[TT_MAX_SPLITS];
-        float4 x[TT_MAX_SPLITS][2];
-        float top = -INFINITY, sum = 0.f, o[8];
+        float4 x[TT_MAX_SPLITS][COLS / 4];
+        float top = -INFINITY, sum = 0.f, o[COLS];
 #pragma unroll
         for (int p = 0; p < TT_MAX_SPLITS; ++p) {
           ps[p] = make_float2(-INFINITY, 0.f);
           if (p >= splits) continue;
           ps[p] = peer_load2(peer_u32(ml + mine, p));
 #pragma unroll
-          for (int d = 0; d < 2; ++d)
+          for (int d = 0; d < COLS / 4; ++d)
             x[p][d] = peer_load4(peer_u32(part_piece<64, D>(p_sm + t * P_BYTES, q_sm + t * Q_BYTES, r, c / 4 + d), p));
         }
 #pragma unroll
         for (int p = 0; p < TT_MAX_SPLITS; ++p)
           if (ps[p].y != 0.f) top = fmaxf(top, ps[p].x);
 #pragma unroll
-        for (int d = 0; d < 8; ++d) o[d] = 0.f;
+        for (int d = 0; d < COLS; ++d) o[d] = 0.f;
 #pragma unroll
         for (int p = 0; p < TT_MAX_SPLITS; ++p) {
           // (a part whose sum is no number has a score that is none, which is the row's result)
@@ -467,7 +469,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
           const float w = fast_exp2(ps[p].x - top);
           sum = fmaf(w, ps[p].y, sum);
 #pragma unroll
-          for (int d = 0; d < 2; ++d) {
+          for (int d = 0; d < COLS / 4; ++d) {
             o[4 * d] = fmaf(w, x[p][d].x, o[4 * d]); o[4 * d + 1] = fmaf(w, x[p][d].y, o[4 * d + 1]);
             o[4 * d + 2] = fmaf(w, x[p][d].z, o[4 * d + 2]); o[4 * d + 3] = fmaf(w, x[p][d].w, o[4 * d + 3]);
           }
@@ -476,7 +478,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
         const int row = row0 + mine;
         bf16* dst = (bf16*)a.out + ((size_t)(start + row / group) * a.heads + kvh * group + row % group) * D + c;
 #pragma unroll
-        for (int d = 0; d < 8; d += 4) {
+        for (int d = 0; d < COLS; d += 4) {
           const __nv_bfloat162 two = __floats2bfloat162_rn(o[d] * inv, o[d + 1] * inv), more = __floats2bfloat162_rn(o[d + 2] * inv, o[d + 3] * inv);
           *reinterpret_cast<uint2*>(dst + d) = make_uint2(*reinterpret_cast<const uint32_t*>(&two), *reinterpret_cast<const uint32_t*>(&more));
         }

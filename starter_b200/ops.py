@@ -1407,8 +1407,8 @@ def _tree_mma_plan(rows: int, units: int, keys: int, dim: int) -> tuple:
     """``(row warps, splits)`` of the mma.sync kernel for ``rows`` packed rows of each of ``units`` (sequence, key/value head) pairs: tiles of 16
     rows while they are fewer than the SMs, of 32 behind that (a tile reads all keys), and as many parts of the keys as blocks run at once, two
     an SM (four of heads of up to 64).  Measured (us, heads of 128): 8 pairs of 64 rows behind 1,500 tokens in tiles of 16 / 32 rows, 8
-    parts, 9.4 / 11.4; 128 pairs of 64 rows 42.1 / 40.9, behind 500 24.8 / 21.7; 32 pairs of 16 rows behind 4,096 in 4 / 6 / 8 parts 21.2 /
-    17.5 / 16.4."""
+    parts, 9.1 / 10.6; 128 pairs of 64 rows 41.6 / 38.0, behind 500 24.1 / 20.0; 32 pairs of 16 rows behind 4,096 in 4 / 6 / 8 parts 20.9 /
+    17.3 / 15.9."""
     row_warps = 1 if rows <= 16 or units * -(-rows // 16) <= SM_COUNT else 2
     blocks = units * -(-rows // (16 * row_warps))
     return row_warps, max(1, min(8, (2 if dim > 64 else 4) * SM_COUNT // blocks, -(-keys // PAGE_TOKENS)))
@@ -1417,11 +1417,11 @@ def _tree_mma_plan(rows: int, units: int, keys: int, dim: int) -> tuple:
 def _tree_on_tmem(rows: int, units: int, keys: int, dim: int) -> bool:
     """Whether the tcgen05 kernel is the faster one, by the scores a step forms.  Its tiles have 128 rows however few are real, and its
     blocks take 8 to 10 us whatever they read; a score costs it less than half.  Measured (us, mma.sync / tcgen05, heads of 128, scores in
-    millions): 16 pairs of 64 rows behind 1,500 tokens (1.5) 12.2 / 13.9, 32 pairs (3.1) 18.3 / 14.7, 64 pairs behind 500 (2.0) 16.1 / 13.9; 16
-    pairs of 32 rows behind 4,096 (2.1) 14.6 / 19.0, 32 pairs (4.2) 22.3 / 20.6; 128 pairs of 16 rows behind 4,096 (8.4) 41.2 / 47.5; two tiles, 8 pairs of
-    256 rows behind 1,500 (3.1) 19.4 / 23.7, 16 pairs (6.1) 26.8 / 25.0.  Heads of 64, where the two are within a tenth of each other around the
-    bounds: 64 pairs of 64 rows behind 500 (2.0) 11.3 / 12.1, 32 behind 1,500 (3.1) 12.0 / 11.1, behind 4,096 64 pairs (16.8) 29.8 / 26.8, 128 pairs of 32
-    rows (16.8) 29.8 / 43.7."""
+    millions): 16 pairs of 64 rows behind 1,500 tokens (1.5) 11.9 / 13.5, 32 pairs (3.1) 17.8 / 14.3, 64 pairs behind 500 (2.0) 15.4 / 14.2; 16
+    pairs of 32 rows behind 4,096 (2.1) 14.5 / 18.3, 32 pairs (4.2) 22.1 / 19.6; 128 pairs of 16 rows behind 4,096 (8.4) 40.6 / 47.8; two tiles, 8 pairs of
+    256 rows behind 1,500 (3.1) 19.0 / 24.2, 16 pairs (6.1) 25.2 / 23.3.  Heads of 64, where the two are within a tenth of each other around the
+    bounds: 64 pairs of 64 rows behind 500 (2.0) 11.2 / 12.2, 32 behind 1,500 (3.1) 11.5 / 10.8, behind 4,096 64 pairs (16.8) 29.6 / 26.6, 128 pairs of 32
+    rows (16.8) 30.0 / 43.1."""
     if rows <= (16 if dim > 64 else 32):
         return False
     return units * rows * keys > (5_500_000 if rows > 128 else 2_000_000 if units >= 64 else 3_000_000)
@@ -1438,8 +1438,8 @@ def _tree_tc_clusters(size: int, device: int) -> int:
 @functools.lru_cache(maxsize=4096)
 def _tree_tc_splits(blocks: int, keys: int, device: int) -> int:
     """How many CTAs share the keys of a block of 256 rows: as many as run at once, with 170 keys or more each.  Measured (us in 1 / 2 / 4 / 8
-    parts, 64 rows of 8 pairs, heads of 64): behind 1,500 tokens 18.4 / 14.0 / 10.4 / 9.3, behind 4,096 41.8 / 25.2 / 16.1 / 11.8; 64 pairs of 256 rows of
-    128 behind 4,096, which run at once in up to 2 parts, 66.5 / 47.6 / 56.8."""
+    parts, 64 rows of 8 pairs, heads of 64): behind 1,500 tokens 18.1 / 13.9 / 10.3 / 9.3, behind 4,096 40.5 / 25.0 / 16.0 / 11.8; 64 pairs of 256 rows of
+    128 behind 4,096, which run at once in up to 2 parts, 63.3 / 44.3 / 53.3."""
     return next((parts for parts in (8, 4, 2) if keys >= max(800, 170 * parts) and blocks <= _tree_tc_clusters(parts, device)), 1)
 
 
