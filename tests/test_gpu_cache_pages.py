@@ -153,6 +153,16 @@ def test_accepted_rows_past_two_to_the_31_entries():
     assert torch.equal(wide[0][:, shift], before) and torch.equal(wide[0][:, shift + 1], before)
 
 
+def test_accept_where_new_memory_has_to_be_filled():
+    """Deterministic algorithms fill what is allocated: the results are separate tensors then, with the same contents."""
+    was = torch.are_deterministic_algorithms_enabled()
+    torch.use_deterministic_algorithms(True)
+    try:
+        Step([20, 33], [100, 7], vocab=2, seed=7).check()
+    finally:
+        torch.use_deterministic_algorithms(was)
+
+
 def test_accept_refusals():
     s = Step([8], [50])
     k, v = s.keys.cuda(), s.values.cuda()
