@@ -269,35 +269,52 @@ PyObject* empty(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return out;
 }
 
-// empties(like, shape, shape, ...): small results of like's type, together in one allocation (each on a boundary of 16 bytes), or one by one.
+// empties(like, shape | dtype, ...): small results of one call together in one allocation (each on a boundary of 64 bytes), or one by one; a dtype
+// is that of the shapes behind it, like's at first.
 PyObject* empties(PyObject* self, PyObject* const* args, Py_ssize_t n) {
-  if (n < 2 || n > 9 || !THPVariable_Check(args[0])) {
-    PyErr_SetString(PyExc_TypeError, "empties(like, shape, ...) of up to eight shapes");
+  constexpr int MOST = 8;
+  PyObject* shapes[MOST];
+  PyObject* types[MOST];
+  int count = 0;
+  PyObject* type = Py_None;
+  bool valid = n >= 2 && THPVariable_Check(args[0]);
+  for (Py_ssize_t i = 1; i < n && valid; ++i) {
+    if (THPDtype_Check(args[i])) {
+      type = args[i];
+    } else if ((valid = count < MOST && PyTuple_Check(args[i]))) {
+      shapes[count] = args[i];
+      types[count++] = type;
+    }
+  }
+  if (!valid) {
+    PyErr_SetString(PyExc_TypeError, "empties(like, shape or dtype, ...) of up to eight shapes");
     return nullptr;
   }
-  PyObject* out = PyTuple_New(n - 1);
+  PyObject* out = PyTuple_New(count);
   if (!out) return nullptr;
   const at::Tensor& like = THPVariable_Unpack(args[0]);
   if (like.is_cuda() && !at::globalContext().deterministicAlgorithms()) {
     try {
-      int64_t sizes[8][6], first[8], total = 0;
+      int64_t sizes[MOST][6], first[MOST], total = 0;
+      at::ScalarType scalar[MOST];
       bool plain = true;
-      for (Py_ssize_t i = 0; i + 1 < n && plain; ++i) {
-        plain = PyTuple_Check(args[i + 1]) && PyTuple_GET_SIZE(args[i + 1]) <= 6 && sizes_of(args[i + 1], sizes[i]);
-        int64_t count = 1;
-        for (Py_ssize_t d = 0; plain && d < PyTuple_GET_SIZE(args[i + 1]); ++d) {
-          plain = sizes[i][d] >= 0 && (sizes[i][d] == 0 || count <= (int64_t(1) << 40) / sizes[i][d]);
-          count *= plain ? sizes[i][d] : 0;
+      for (int i = 0; i < count && plain; ++i) {
+        scalar[i] = types[i] == Py_None ? like.scalar_type() : reinterpret_cast<THPDtype*>(types[i])->scalar_type;
+        plain = PyTuple_GET_SIZE(shapes[i]) <= 6 && sizes_of(shapes[i], sizes[i]);
+        int64_t bytes = c10::elementSize(scalar[i]);
+        for (Py_ssize_t d = 0; plain && d < PyTuple_GET_SIZE(shapes[i]); ++d) {
+          plain = sizes[i][d] >= 0 && (sizes[i][d] == 0 || bytes <= (int64_t(1) << 44) / sizes[i][d]);
+          bytes *= plain ? sizes[i][d] : 0;
         }
         first[i] = total;
-        total += (count + 15) / 16 * 16;
+        total += (bytes + 63) / 64 * 64;
       }
       if (plain) {
-        const at::Tensor all = at::detail::empty_cuda(at::IntArrayRef(&total, 1), like.scalar_type(), like.device(), std::nullopt);
-        for (Py_ssize_t i = 0; i + 1 < n; ++i) {
-          at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), all.dtype());
-          t.unsafeGetTensorImpl()->set_storage_offset(first[i]);
-          t.unsafeGetTensorImpl()->set_sizes_contiguous(at::IntArrayRef(sizes[i], PyTuple_GET_SIZE(args[i + 1])));
+        const at::Tensor all = at::detail::empty_cuda(at::IntArrayRef(&total, 1), at::kByte, like.device(), std::nullopt);
+        for (int i = 0; i < count; ++i) {
+          at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), c10::scalarTypeToTypeMeta(scalar[i]));
+          t.unsafeGetTensorImpl()->set_storage_offset(first[i] / (int64_t)c10::elementSize(scalar[i]));
+          t.unsafeGetTensorImpl()->set_sizes_contiguous(at::IntArrayRef(sizes[i], PyTuple_GET_SIZE(shapes[i])));
           PyObject* wrapped = THPVariable_Wrap(std::move(t));
           if (!wrapped) {
             Py_DECREF(out);
@@ -308,15 +325,15 @@ PyObject* empties(PyObject* self, PyObject* const* args, Py_ssize_t n) {
         return out;
       }
     } catch (const std::exception&) {
-      for (Py_ssize_t i = 0; i + 1 < n; ++i) {
+      for (int i = 0; i < count; ++i) {
         Py_XDECREF(PyTuple_GET_ITEM(out, i));
         PyTuple_SET_ITEM(out, i, nullptr);
       }
     }
   }
-  for (Py_ssize_t i = 0; i + 1 < n; ++i) {
-    PyObject* one[2] = {args[0], args[i + 1]};
-    PyObject* made = empty(self, one, 2);
+  for (int i = 0; i < count; ++i) {
+    PyObject* one[3] = {args[0], shapes[i], types[i]};
+    PyObject* made = empty(self, one, 3);
     if (!made) {
       Py_DECREF(out);
       return nullptr;
@@ -324,6 +341,53 @@ PyObject* empties(PyObject* self, PyObject* const* args, Py_ssize_t n) {
     PyTuple_SET_ITEM(out, i, made);
   }
   return out;
+}
+
+// The tensor behind an argument if it is of this type and number of dimensions, contiguous and on the current device; nullptr otherwise.
+const at::Tensor* fitting(PyObject* o, at::ScalarType type, int64_t dims) {
+  if (!THPVariable_Check(o)) return nullptr;
+  const at::Tensor& t = THPVariable_Unpack(o);
+  return t.scalar_type() == type && t.dim() == dims && here(t) ? &t : nullptr;
+}
+
+// step_fits(block_table, vector, ...): how many sequences a step's int32 arrays describe (a table, and vectors of one length); -1 where one does not fit.
+PyObject* step_fits(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  try {
+    long long seqs = -1;
+    if (n < 2 || !fitting(args[0], at::kInt, 2)) return PyLong_FromLong(-1);
+    for (Py_ssize_t i = 1; i < n; ++i) {
+      const at::Tensor* t = fitting(args[i], at::kInt, 1);
+      if (!t || (seqs >= 0 && t->size(0) != seqs)) return PyLong_FromLong(-1);
+      seqs = t->size(0);
+    }
+    return PyLong_FromLongLong(seqs);
+  } catch (const std::exception&) {
+    return PyLong_FromLong(-1);
+  }
+}
+
+// tree_rows(q, keys, values, tok_pos, tree_mask, width, kv_heads, page, head_dim): how many nodes an attention's operands describe; -1 where one does not fit.
+PyObject* tree_rows(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  long long want[4];
+  if (n != 9 || !THPVariable_Check(args[0])) return PyLong_FromLong(-1);
+  for (int i = 0; i < 4; ++i) {
+    want[i] = PyLong_AsLongLong(args[5 + i]);
+    if (want[i] == -1 && PyErr_Occurred()) {
+      PyErr_Clear();
+      return PyLong_FromLong(-1);
+    }
+  }
+  try {
+    const at::ScalarType type = THPVariable_Unpack(args[0]).scalar_type();
+    const at::Tensor *q = fitting(args[0], type, 2), *k = fitting(args[1], type, 4), *v = fitting(args[2], type, 4), *pos = fitting(args[3], at::kInt, 1),
+                     *mask = fitting(args[4], at::kInt, 2);
+    if (!q || !k || !v || !pos || !mask || q->size(1) != want[0] || pos->size(0) != q->size(0) || mask->size(0) != q->size(0)) return PyLong_FromLong(-1);
+    for (const at::Tensor* t : {k, v})
+      if (t->size(1) != want[1] || t->size(2) != want[2] || t->size(3) != want[3]) return PyLong_FromLong(-1);
+    return PyLong_FromLongLong(q->size(0));
+  } catch (const std::exception&) {
+    return PyLong_FromLong(-1);
+  }
 }
 
 // Whether an operation on these tensors would go straight to its CUDA kernel: plain tensors, nothing recorded, cast, mapped or traced.
@@ -472,6 +536,8 @@ PyMethodDef methods[] = {
     {"page_rows", (PyCFunction)(void (*)(void))page_rows, METH_FASTCALL, nullptr},
     {"empty", (PyCFunction)(void (*)(void))empty, METH_FASTCALL, nullptr},
     {"empties", (PyCFunction)(void (*)(void))empties, METH_FASTCALL, nullptr},
+    {"step_fits", (PyCFunction)(void (*)(void))step_fits, METH_FASTCALL, nullptr},
+    {"tree_rows", (PyCFunction)(void (*)(void))tree_rows, METH_FASTCALL, nullptr},
     {"product", (PyCFunction)(void (*)(void))product, METH_FASTCALL, nullptr},
     {"block_steps", (PyCFunction)(void (*)(void))block_steps, METH_FASTCALL, nullptr},
     {"mixed_splits", (PyCFunction)(void (*)(void))mixed_splits, METH_FASTCALL, nullptr},

@@ -94,12 +94,13 @@ def _refuse(t, name, dtype=None, ndim=None):
 # launch, are native too (csrc/host.cpp).  The first call of any of them loads the native part and puts it in these names.
 
 def _bind():
-    global _need, _fits, _empty, _empties, _items, _page_rows, _stream, _product, _block_steps, _mixed_splits
+    global _need, _fits, _empty, _empties, _items, _page_rows, _step_fits, _tree_rows, _stream, _product, _block_steps, _mixed_splits
     host = build.load_host()
     host.refuse_with(_refuse)
     _need, _fits, _empty, _stream, _product = host.need, host.fits, host.empty, host.stream, host.product
     _block_steps, _mixed_splits = host.block_steps, host.mixed_splits
     _empties, _items, _page_rows = host.empties, host.items, host.page_rows
+    _step_fits, _tree_rows = host.step_fits, host.tree_rows
     return host
 
 
@@ -120,8 +121,22 @@ def _empty(like, shape, dtype=None):
 
 
 def _empties(like, *shapes):
-    """Small results of one call, in one allocation."""
+    """Small results of one call, in one allocation (a dtype among the shapes is that of those behind it)."""
     return _bind().empties(like, *shapes)
+
+
+def _step_fits(block_table, *vectors):
+    """How many sequences a step's int32 arrays describe: a table and vectors of one length; -1 where one does not fit."""
+    if not all(isinstance(t, torch.Tensor) and t.is_cuda for t in (block_table, *vectors)):
+        return -1                          # (what is refused needs no native part)
+    return _bind().step_fits(block_table, *vectors)
+
+
+def _tree_rows(q, keys, values, tok_pos, tree_mask, *sizes):
+    """How many nodes the operands of ``attention_tree`` describe; -1 where one does not fit."""
+    if not all(isinstance(t, torch.Tensor) and t.is_cuda for t in (q, keys, values, tok_pos, tree_mask)):
+        return -1
+    return _bind().tree_rows(q, keys, values, tok_pos, tree_mask, *sizes)
 
 
 def _items(t, dim):
@@ -1297,8 +1312,7 @@ def token_logprobs(logits, tokens, top=0, status=None):
     if top and vocab * item > 4 * LOGPROBS_MAX_VOCAB:
         raise KernelError(f"alternatives of rows of {vocab} entries; {4 * LOGPROBS_MAX_VOCAB // item} are the most")
     code = _code(logits.dtype)
-    given, entropy = _empty(tokens, (rows,), torch.float32), _empty(tokens, (rows,), torch.float32)
-    values, ids = _empty(tokens, (rows, top), torch.float32), _empty(tokens, (rows, top))
+    given, entropy, values, ids = _empties(tokens, torch.float32, (rows,), (rows,), (rows, top), torch.int32, (rows, top))
     if rows:
         whole, parts = _logprob_plan(rows, vocab * item)
         rc = _lib("token_logprobs").sb_token_logprobs(
@@ -1343,7 +1357,7 @@ def linear_logprobs(h, weight, tokens, cap=None, status=None, withhold=None):
         raise KernelError(f"{tokens.shape[0]} tokens for {rows} rows")
     if vocab == 0 or h.shape[1] == 0:
         raise KernelError(f"a head of shape {tuple(weight.shape)} gives no logits")
-    given, entropy = _empty(h, (rows,), torch.float32), _empty(h, (rows,), torch.float32)
+    given, entropy = _empties(h, torch.float32, (rows,), (rows,))
     if cap is not None and not cap > 0:
         raise KernelError(f"a cap of {cap}")
     if h.dtype == torch.bfloat16 and rows > TENSOR_CORE_MAX_ROWS and h.shape[1] % 8 == 0 and not (h.data_ptr() | weight.data_ptr()) & 15:
@@ -1372,15 +1386,6 @@ def linear_logprobs(h, weight, tokens, cap=None, status=None, withhold=None):
 
 #: the most nodes a sequence's tree may have
 TREE_MAX_NODES = 256
-
-
-def _tree_step_fits(block_table, seq_slot, seq_q_start, seq_q_len, seq_kv_len, max_q_len):
-    """How many sequences a step's arrays describe, or None where something about them is wrong."""
-    if not (_fits(seq_slot, torch.int32, None) and _fits(block_table, torch.int32, None, None) and 1 <= max_q_len <= TREE_MAX_NODES):
-        return None
-    seqs = seq_slot.shape[0]
-    fits = _fits(seq_q_start, torch.int32, seqs) and _fits(seq_q_len, torch.int32, seqs) and _fits(seq_kv_len, torch.int32, seqs)
-    return seqs if fits else None
 
 
 def _refuse_tree_step(block_table, seq_slot, seq_q_start, seq_q_len, seq_kv_len, max_q_len):
@@ -1464,18 +1469,14 @@ def attention_tree(q, k_store, v_store, block_table, seq_slot, seq_q_start, seq_
     ``limit_ns``, bit 16 of ``status`` is set and the result is undefined."""
     if max_q_len is None:
         max_q_len = min(32 * tree_mask.shape[1], TREE_MAX_NODES) if isinstance(tree_mask, torch.Tensor) and tree_mask.dim() == 2 else 0
-    seqs, dtype = None, getattr(q, "dtype", None)
-    if _fits(q, None, None, heads * head_dim) and _fits(k_store, dtype, None, kv_heads, PAGE_TOKENS, head_dim) \
-            and _fits(v_store, dtype, None, kv_heads, PAGE_TOKENS, head_dim):
-        rows = q.shape[0]
-        if _fits(tok_pos, torch.int32, rows) and _fits(tree_mask, torch.int32, rows, None):
-            seqs = _tree_step_fits(block_table, seq_slot, seq_q_start, seq_q_len, seq_kv_len, max_q_len)
-    if seqs is None or kv_heads < 1 or heads % kv_heads or not 1 <= head_dim <= MAX_HEAD_DIM or (window is not None and window < 1) \
-            or 32 * tree_mask.shape[1] < max_q_len:
+    rows = _tree_rows(q, k_store, v_store, tok_pos, tree_mask, heads * head_dim, kv_heads, PAGE_TOKENS, head_dim)
+    seqs = _step_fits(block_table, seq_slot, seq_q_start, seq_q_len, seq_kv_len)
+    if rows < 0 or seqs < 0 or not 1 <= max_q_len <= TREE_MAX_NODES or kv_heads < 1 or heads % kv_heads or not 1 <= head_dim <= MAX_HEAD_DIM \
+            or (window is not None and window < 1) or 32 * tree_mask.shape[1] < max_q_len:
         _refuse_tree(q, k_store, v_store, tok_pos, tree_mask, heads, kv_heads, head_dim, window)
         _refuse_tree_step(block_table, seq_slot, seq_q_start, seq_q_len, seq_kv_len, max_q_len)
         raise KernelError(f"masks of {tree_mask.shape[1]} words for trees of {max_q_len} nodes")
-    code, words = _code(dtype), tree_mask.shape[1]
+    code, words = _code(q.dtype), tree_mask.shape[1]
     out = _empty(q, (rows, heads * head_dim))
     if rows == 0 or seqs == 0:
         return out
@@ -1547,9 +1548,8 @@ def cache_accept(stores, block_table, seq_slot, seq_q_start, seq_q_len, seq_kv_l
     dimension).  Returns int32 ``count`` ``[S]`` (nodes on the way), ``path`` ``[S, max_q_len]`` (which ones, then -1) and ``taken``
     ``[S, max_q_len]`` (what was drawn at each, then -1): the sequence has ``past + count`` tokens now and goes on with
     ``taken[count - 1]``.  ``max_q_len``: the longest ``seq_q_len``, at most ``TREE_MAX_NODES``."""
-    seqs = _tree_step_fits(block_table, seq_slot, seq_q_start, seq_q_len, seq_kv_len, max_q_len)
-    if seqs is None or not (_fits(tokens, torch.int32, None) and _fits(parents, torch.int32, tokens.shape[0])
-                            and _fits(drawn, torch.int32, tokens.shape[0])):
+    seqs = _step_fits(block_table, seq_slot, seq_q_start, seq_q_len, seq_kv_len)
+    if seqs < 0 or not 1 <= max_q_len <= TREE_MAX_NODES or _step_fits(block_table, tokens, parents, drawn) < 0:
         _refuse_tree_step(block_table, seq_slot, seq_q_start, seq_q_len, seq_kv_len, max_q_len)
         for name, t in (("tokens", tokens), ("parents", parents), ("drawn", drawn)):
             _need(t, name, torch.int32, 1)
