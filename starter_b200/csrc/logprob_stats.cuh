@@ -6,11 +6,12 @@
 
 struct Stats { float m, l, t; };
 
-__device__ __forceinline__ float lp_exp(float d) {
+__device__ __forceinline__ float lp_exp2(float x) {
   float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(d * 1.4426950408889634f));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float lp_exp(float d) { return lp_exp2(d * 1.4426950408889634f); }
 // Both parts on the larger reference.  (A part that has seen no finite entry has m = -inf, L = T = 0.)
 __device__ __forceinline__ Stats lp_join(const Stats& a, const Stats& b) {
   const float m = fmaxf(a.m, b.m), base = m == -INFINITY ? 0.f : m;
