@@ -357,7 +357,7 @@ int sb_attention_tree_plain(int dtype, const void* q, void* out, const void* k_s
   if (kv_heads <= 0 || heads % kv_heads || dim < 1 || dim > 256 || words < 1 || splits < 1 || splits > TP_CLUSTER_MAX) return -2;
   if ((long long)seqs * kv_heads > 65535 || max_q_len > 32 * TREE_MAX_WORDS) return -2;
   const TreeArgs a{q, out, k_store, v_store, block_table, table_stride, seq_slot, seq_q_start, seq_q_len, seq_kv_len, tok_pos,
-                   (const uint32_t*)mask, words < TREE_MAX_WORDS ? words : TREE_MAX_WORDS, heads, kv_heads, dim, scale * 1.4426950408889634f,
+                   (const uint32_t*)mask, words, words < TREE_MAX_WORDS ? words : TREE_MAX_WORDS, heads, kv_heads, dim, scale * 1.4426950408889634f,
                    window > 0 ? window : 0, splits};
   if (dtype == 0) return dim <= 128 ? launch_plain<float, 1>(a, seqs, max_q_len, s) : launch_plain<float, 2>(a, seqs, max_q_len, s);
   if (dtype == 1) return dim <= 128 ? launch_plain<bf16, 1>(a, seqs, max_q_len, s) : launch_plain<bf16, 2>(a, seqs, max_q_len, s);

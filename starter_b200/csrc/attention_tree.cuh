@@ -24,8 +24,8 @@ struct TreeArgs {
   const int* seq_q_len;
   const int* seq_kv_len;
   const int* tok_pos;        // [tokens]
-  const uint32_t* mask;      // [tokens, words]
-  int words;
+  const uint32_t* mask;      // [tokens, mask_stride]
+  int mask_stride, words;    // words a row holds; those of them that nodes can have (at most TREE_MAX_WORDS)
   int heads, kv_heads, dim;
   float scale_log2;          // scale * log2(e): exponentials are powers of two
   int window;                // 0: none
@@ -70,7 +70,7 @@ __device__ __forceinline__ int tree_low(const TreeArgs& a, int past) { return a.
 __device__ __forceinline__ int tree_high(const TreeArgs& a, int past, int kv_len) { return a.window > 0 ? min(max(kv_len - a.window, 0), past) : 0; }
 // Word w of the mask of a sequence's node, without the nodes in front of its window (first: its first place; up to `past` it leaves out none).
 __device__ __forceinline__ uint32_t tree_mask_word(const TreeArgs& a, int start, int node, int w, int q_len, int first, int past) {
-  uint32_t bits = w < a.words ? a.mask[(size_t)(start + node) * a.words + w] : 0u;
+  uint32_t bits = w < a.words ? a.mask[(size_t)(start + node) * a.mask_stride + w] : 0u;
   if (a.window > 0 && first > past) {
     for (uint32_t left = bits; left; left &= left - 1) {
       const int m = 32 * w + __ffs(left) - 1;

@@ -420,7 +420,7 @@ int sb_attention_tree_mma(const void* q, void* out, const void* k_store, const v
   if ((long long)seqs * kv_heads > 65535 || max_q_len > TM_MAX_NODES) return -2;
   if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_store | (uintptr_t)v_store) & 15) return -2;
   const TreeArgs a{q, out, k_store, v_store, block_table, table_stride, seq_slot, seq_q_start, seq_q_len, seq_kv_len, tok_pos,
-                   (const uint32_t*)mask, words < TREE_MAX_WORDS ? words : TREE_MAX_WORDS, heads, kv_heads, dim,
+                   (const uint32_t*)mask, words, words < TREE_MAX_WORDS ? words : TREE_MAX_WORDS, heads, kv_heads, dim,
                    scale * 1.4426950408889634f, window > 0 ? window : 0, splits};
   switch (dim) {
     case 16: return launch<16>(a, seqs, max_q_len, row_warps, s);

@@ -559,7 +559,7 @@ int sb_attention_tree_tc(const void* q, void* out, const void* k_store, const vo
   rc = sb_make_map(&mv, v_store, kv_rows, dim, SB_PAGE_TOKENS);
   if (rc) return rc;
   const TreeArgs a{q, out, k_store, v_store, block_table, table_stride, seq_slot, seq_q_start, seq_q_len, seq_kv_len, tok_pos,
-                   (const uint32_t*)mask, words < TREE_MAX_WORDS ? words : TREE_MAX_WORDS, heads, kv_heads, dim,
+                   (const uint32_t*)mask, words, words < TREE_MAX_WORDS ? words : TREE_MAX_WORDS, heads, kv_heads, dim,
                    scale * 1.4426950408889634f, window > 0 ? window : 0, splits};
   const bool test_run = next_withhold_step >= 0;
   if (test_run) {

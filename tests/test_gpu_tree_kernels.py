@@ -1,0 +1,46 @@
+"""Tree attention on each of its kernels by name, with keys whole and in parts: the cases that a step's size alone would send to one of them only."""
+
+import math
+import threading
+
+import pytest
+import torch
+
+from starter_b200 import ops
+from test_gpu_tree_attention import PAGE, Case, bush, chain, check, depth_of, sees_of, trees
+
+pytestmark = pytest.mark.gpu
+
+#: kernel, type, head size, parts
+FORMS = [("plain", "fp32", 64, 1), ("plain", "fp32", 128, 4), ("plain", "bf16", 80, 3), ("plain", "bf16", 7, 1),
+         ("mma", "bf16", 32, (1, 1)), ("mma", "bf16", 64, (2, 4)), ("mma", "bf16", 128, (2, 1)), ("mma", "bf16", 128, (1, 8)),
+         ("tcgen05", "bf16", 64, 1), ("tcgen05", "bf16", 64, 4), ("tcgen05", "bf16", 128, 1), ("tcgen05", "bf16", 128, 2), ("tcgen05", "bf16", 128, 8)]
+every_kernel = pytest.mark.parametrize("kernel, dtype, dim, parts", FORMS, ids=lambda v: str(v).replace(" ", ""))
+
+
+def run(case, kernel, parts, **more):
+    return ops.attention_tree(**{**case.on_device(), "kernel": kernel, "parts": parts, **more})
+
+
+def spoil(case, seq, place, what, column=2, kv_head=0, which="v"):
+    """Put what is no number at a place of a sequence's values (or keys)."""
+    getattr(case, which)[int(case.table[case.slots[seq], place // PAGE]), kv_head, place % PAGE, column] = what
+
+
+def check_finite(case, got):
+    """Numbers within the bound, and none where a row sees a value that is none."""
+    want, tol = case.want()
+    got = got.double().cpu()
+    fine = torch.isfinite(want)
+    assert torch.equal(torch.isfinite(got), fine), f"first at {(torch.isfinite(got) != fine).nonzero()[0].tolist()}"
+    assert ((got - want).abs()[fine] <= tol[fine]).all()
+
+
+@every_kernel
+@pytest.mark.parametrize("words", [2, 8, 9, 11])
+def test_masks_wider_than_a_tree(kernel, dtype, dim, parts, words):
+    """Words behind those that the nodes need, whatever their bits say."""
+    sees, depth = trees([13, 40], seed=words)
+    case = Case(dtype, 4, 2, dim, sees, [70, 131], depth, seed=words, words=words)
+    case.mask[:, 2:] = -1
+    check(case, run(case, kernel, parts))
