@@ -1273,17 +1273,19 @@ LOGPROBS_MAX_VOCAB = 8 * 160 * 4096 - 32
 
 
 @functools.lru_cache(maxsize=4096)
-def _logprob_plan(rows: int, row_bytes: int) -> tuple:
+def _logprob_plan(rows: int, row_bytes: int, listed: bool = True) -> tuple:
     """``(whole, parts)``: how many rows of logits have a block of their own, and how many blocks (a cluster) share each of the others.
 
     Four blocks run on an SM.  Full waves of them take whole rows; what is left over is cut so that it fills the SMs once more, down to
-    two of a block's tiles of 16 KB, and runs into the last wave's end."""
+    two of a block's tiles of 16 KB, and runs into the last wave's end.  With alternatives (``listed``) a block holds the groups of 160
+    tiles.  Tiles begin on 32-byte boundaries and rows anywhere, so what may lie in front of a row counts there, as it does in the launcher."""
     places, tiles = 4 * SM_COUNT, -(-row_bytes // 16384)
+    held = -(-(row_bytes + 31) // 16384) if listed else tiles
     left, parts = rows % places, 1
     while parts < 8 and 2 * parts * left <= places and 4 * parts <= tiles:
         parts *= 2
-    if tiles > 160:                          # (more than a block's shared memory holds the groups of)
-        while -(-tiles // parts) > 160:
+    if held > 160:
+        while -(-held // parts) > 160:
             parts *= 2
         return 0, parts
     return (rows if left == 0 or parts == 1 else rows - left), parts
@@ -1314,7 +1316,7 @@ def token_logprobs(logits, tokens, top=0, status=None):
     code = _code(logits.dtype)
     given, entropy, values, ids = _empties(tokens, torch.float32, (rows,), (rows,), (rows, top), torch.int32, (rows, top))
     if rows:
-        whole, parts = _logprob_plan(rows, vocab * item)
+        whole, parts = _logprob_plan(rows, vocab * item, top > 0)
         rc = _lib("token_logprobs").sb_token_logprobs(
             code, logits, rows, vocab, logits.stride(0), tokens, top, given, entropy, values, ids, whole, parts, status, _stream())
         _check(rc, "token_logprobs", 2 if 0 < whole < rows else 1)
