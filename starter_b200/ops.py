@@ -1285,7 +1285,7 @@ def _logprob_plan(rows: int, row_bytes: int, listed: bool = True) -> tuple:
     while parts < 8 and 2 * parts * left <= places and 4 * parts <= tiles:
         parts *= 2
     if held > 160:
-        while -(-held // parts) > 160:
+        while parts < 8 and -(-held // parts) > 160:          # (a longer row than eight hold lists none)
             parts *= 2
         return 0, parts
     return (rows if left == 0 or parts == 1 else rows - left), parts

@@ -28,3 +28,8 @@ def check_rows(x, t, top, step=50):
 def test_alternatives_where_a_block_has_as_many_tiles_as_it_holds(dtype, rows, vocab):
     x, t = logits(rows, vocab, vocab, dtype)
     check_rows(x, t, 3)
+
+
+@pytest.mark.parametrize("dtype, rows, vocab", [(torch.float32, 2, 5_300_000), (torch.float32, 40, 5_242_900), (torch.bfloat16, 2, 10_600_001)])
+def test_rows_longer_than_alternatives_take(dtype, rows, vocab):
+    check_rows(*logits(rows, vocab, vocab, dtype), 0)

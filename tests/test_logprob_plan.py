@@ -37,3 +37,11 @@ def test_rows_with_alternatives_fit_what_a_block_holds(item, rows):
             assert launched_tiles(vocab, item, parts) <= MOST_TILES, (rows, vocab, parts)
         if whole:
             assert launched_tiles(vocab, item, 1) <= MOST_TILES, (rows, vocab)
+
+
+@pytest.mark.parametrize("item", [2, 4])
+@pytest.mark.parametrize("rows", [1, 2, 75, 300, 592, 600])
+def test_rows_of_any_length_without_alternatives_have_a_plan(item, rows):
+    for vocab in (5_242_848, 5_242_881, 10_485_761, 20_000_000, 2 ** 30):
+        whole, parts = ops._logprob_plan(rows, vocab * item, False)
+        assert parts in (1, 2, 4, 8) and parts <= MOST_PARTS and 0 <= whole <= rows
