@@ -1597,17 +1597,18 @@ def cache_copy_pages(stores, source, target, dim=1):
 
     ``stores`` are contiguous tensors of a cache group's storage ``[entries, pages, ...]``; ``dim`` says which dimension counts the pages (0:
     one entry's ``[pages, ...]``, or a state ``[slots, ...]``).  No target may be named twice or be a source: the copies are made in any order."""
-    pairs, n = array.array("i"), len(target)
+    pairs = array.array("i")
     try:
+        given, n = len(source), len(target)
         for a, b in zip(source, target):
             pairs.append(a)
             pairs.append(b)
     except (TypeError, OverflowError) as wrong:
         raise KernelError(f"pages are numbered by integers: {wrong}") from None
-    if len(source) != n:
-        raise KernelError(f"{len(source)} pages to copy to {n}")
-    numbers = set(target)
-    if len(numbers) < n or not numbers.isdisjoint(source):
+    if given != n:
+        raise KernelError(f"{given} pages to copy to {n}")
+    numbers = set(pairs[1::2])               # (the numbers themselves: entries of a tensor are all different things)
+    if len(numbers) < n or not numbers.isdisjoint(pairs[::2]):
         raise KernelError("a page is copied to twice, or from and to")
     if dim not in (0, 1):
         raise KernelError(f"pages are counted by the first or the second dimension, not {dim}")
