@@ -382,6 +382,7 @@ PyObject* tree_rows(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const at::Tensor *q = fitting(args[0], type, 2), *k = fitting(args[1], type, 4), *v = fitting(args[2], type, 4), *pos = fitting(args[3], at::kInt, 1),
                      *mask = fitting(args[4], at::kInt, 2);
     if (!q || !k || !v || !pos || !mask || q->size(1) != want[0] || pos->size(0) != q->size(0) || mask->size(0) != q->size(0)) return PyLong_FromLong(-1);
+    if (k->size(0) != v->size(0)) return PyLong_FromLong(-1);      // (one table numbers the pages of both)
     for (const at::Tensor* t : {k, v})
       if (t->size(1) != want[1] || t->size(2) != want[2] || t->size(3) != want[3]) return PyLong_FromLong(-1);
     return PyLong_FromLongLong(q->size(0));

@@ -1529,6 +1529,8 @@ def _refuse_tree(q, k_store, v_store, tok_pos, tree_mask, heads, kv_heads, head_
         _need(store, "cache pages", q.dtype, 4)
         if tuple(store.shape[1:]) != (kv_heads, PAGE_TOKENS, head_dim):
             raise KernelError(f"cache pages have shape {tuple(store.shape)}")
+    if k_store.shape[0] != v_store.shape[0]:
+        raise KernelError(f"{k_store.shape[0]} pages of keys and {v_store.shape[0]} of values")
     _need(tok_pos, "tok_pos", torch.int32, 1)
     _need(tree_mask, "tree_mask", torch.int32, 2)
     for name, t in (("q", q), ("cache pages", k_store), ("cache pages", v_store), ("tok_pos", tok_pos), ("tree_mask", tree_mask)):

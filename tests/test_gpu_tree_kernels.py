@@ -44,3 +44,13 @@ def test_masks_wider_than_a_tree(kernel, dtype, dim, parts, words):
     case = Case(dtype, 4, 2, dim, sees, [70, 131], depth, seed=words, words=words)
     case.mask[:, 2:] = -1
     check(case, run(case, kernel, parts))
+
+
+def test_stores_of_unequal_page_counts_are_refused():
+    """One table numbers the pages of both: a store with fewer would be read behind its end."""
+    sees, depth = trees([5])
+    good = Case("bf16", 4, 2, 64, sees, [100], depth).on_device()
+    for which in ("k_store", "v_store"):
+        for other in (good[which][:-1].contiguous(), torch.cat([good[which], good[which][:1]])):
+            with pytest.raises(ops.KernelError, match="pages of keys"):
+                ops.attention_tree(**{**good, which: other})
