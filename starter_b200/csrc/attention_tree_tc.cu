@@ -78,6 +78,15 @@ __device__ __forceinline__ void tt_load128(uint32_t taddr, float* v) {
   for (int i = 0; i < 128; ++i) v[i] = __uint_as_float(r[i]);
 }
 __device__ __forceinline__ bool tt_no_number(uint32_t half) { return (half & 0x7f80u) == 0x7f80u; }
+// 16 bytes of shared memory that another tile's warps may be writing.
+__device__ __forceinline__ uint4 tt_look(const uint4* p) {
+  uint4 x;
+  asm volatile("ld.relaxed.cta.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(smem_u32(p)));
+  return x;
+}
+__device__ __forceinline__ void tt_put(uint4* p, const uint32_t* w) {
+  asm volatile("st.relaxed.cta.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(smem_u32(p)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+}
 
 // DC: 64-element (128-byte) chunks of a head.
 template <int DC, bool PARTS>
@@ -273,25 +282,38 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
       if (!ok) break;
       if (edge) {
         // Values that are no numbers leave the tile (both tiles' warps may find the same: they write the same zeros).  The buffer's use before is over
-        // (it was the keys of S above, or, for the last values, those of two steps before), so its barrier's parity speaks of this one.
+        // (it was the keys of S above, or, for the last values, those of two steps before), so its barrier's parity speaks of this one.  Whoever finds
+        // zeros where the other tile's warps found such a value has to know at the end that there was one: the flag is set in front of the zeros.
         const int n = v_copy(i);
         ok = together(mbar_wait(&full[n % 3], (n / 3) & 1, abort));
         if (!ok) break;
-        int bad = 0;
-        uint4* v = reinterpret_cast<uint4*>(ring + n % 3 * KV_BYTES);
-#pragma unroll 4
-        for (int idx = (warp & 3) * 32 + lane; idx < DC * SUB / 16; idx += 128) {
-          const uint4 x = v[idx];
-          uint32_t w[4] = {x.x, x.y, x.z, x.w};
-          int here = 0;
+        uint4* v = reinterpret_cast<uint4*>(ring + n % 3 * KV_BYTES) + (warp & 3) * 32 + lane;
+        constexpr int PIECES = DC * SUB / 16 / 128, FLIGHT = 4;
+#pragma unroll 1
+        for (int i0 = 0; i0 < PIECES; i0 += FLIGHT) {
+          uint4 x[FLIGHT];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if (tt_no_number(w[e])) { w[e] &= 0xffff0000u; here = 1; }
-            if (tt_no_number(w[e] >> 16)) { w[e] &= 0xffffu; here = 1; }
+          for (int u = 0; u < FLIGHT; ++u) x[u] = tt_look(v + (i0 + u) * 128);
+          bool here = false;
+#pragma unroll
+          for (int u = 0; u < FLIGHT; ++u)
+            here |= tt_no_number(x[u].x) | tt_no_number(x[u].x >> 16) | tt_no_number(x[u].y) | tt_no_number(x[u].y >> 16) | tt_no_number(x[u].z) |
+                    tt_no_number(x[u].z >> 16) | tt_no_number(x[u].w) | tt_no_number(x[u].w >> 16);
+          if (here) {
+            *(volatile int*)&sh_bad = 1;
+            __threadfence_block();
+#pragma unroll
+            for (int u = 0; u < FLIGHT; ++u) {
+              uint32_t w[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                if (tt_no_number(w[e])) w[e] &= 0xffff0000u;
+                if (tt_no_number(w[e] >> 16)) w[e] &= 0xffffu;
+              }
+              tt_put(v + (i0 + u) * 128, w);
+            }
           }
-          if (here) { v[idx] = make_uint4(w[0], w[1], w[2], w[3]); bad = 1; }
         }
-        if (bad) sh_bad = 1;
       }
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       // The whole row of S first, so that S of the next step can be formed while the exponentials of this one run.
@@ -375,6 +397,11 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_ready[t]);
     }
+    // The tile's warps meet, also those that gave up: what one of them has found all know.
+    __threadfence_block();
+    __syncwarp();
+    if (t) asm volatile("bar.sync 2, 128;" ::: "memory");
+    else asm volatile("bar.sync 1, 128;" ::: "memory");
     if (ok && n_steps > 0) ok = together(mbar_wait(&o_ready[t], (n_steps - 1) & 1, abort));
     if (ok && n_steps > 0) {
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");

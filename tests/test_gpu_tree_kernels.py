@@ -46,6 +46,35 @@ def test_masks_wider_than_a_tree(kernel, dtype, dim, parts, words):
     check(case, run(case, kernel, parts))
 
 
+@every_kernel
+@pytest.mark.parametrize("nodes", [9, 40, 64])
+def test_values_that_are_no_numbers(kernel, dtype, dim, parts, nodes):
+    """In what is cached (every row sees them), at the root, and at leaves that one row each sees: with 40 nodes of 4 heads the last of them lie in
+    the second tile of 128 rows alone."""
+    parents = [-1] + [0] * (nodes - 1)
+    for what, places in ((math.nan, [100 + 5]), (math.inf, [100 + nodes - 1]), (math.nan, [100 + 5, 100 + nodes - 2]), (-math.inf, [100, 100 + 7]),
+                         (math.nan, [99]), (math.inf, [3, 100 + nodes - 1])):
+        case = Case(dtype, 4, 1, dim, [sees_of(parents)], [100], [depth_of(parents)], seed=nodes)
+        for n, place in enumerate(places):
+            spoil(case, 0, place, what, column=(2 + 3 * n) % dim)
+        check_finite(case, run(case, kernel, parts))
+
+
+@pytest.mark.parametrize("dim, parts", [(64, 1), (128, 1), (128, 4)])
+def test_both_tiles_know_of_values_that_are_no_numbers_in_every_run(dim, parts):
+    """Both tiles' warps take the same values out of the shared tile; whoever comes second finds zeros."""
+    parents = [-1] + [0] * 63
+    case = Case("bf16", 8, 2, dim, [sees_of(parents)] * 5, [100, 61, 1, 400, 127], [depth_of(parents)] * 5, seed=dim)
+    for seq, past in enumerate(case.past):
+        for place in range(past, past + 64, 3):
+            spoil(case, seq, place, math.nan, column=place % dim, kv_head=seq % 2)
+    args = case.on_device()
+    first = ops.attention_tree(**args, kernel="tcgen05", parts=parts)
+    check_finite(case, first)
+    for _ in range(200):
+        assert torch.equal(ops.attention_tree(**args, kernel="tcgen05", parts=parts).isnan(), first.isnan())
+
+
 def test_stores_of_unequal_page_counts_are_refused():
     """One table numbers the pages of both: a store with fewer would be read behind its end."""
     sees, depth = trees([5])
