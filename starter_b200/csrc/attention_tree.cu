@@ -185,17 +185,19 @@ __global__ void __launch_bounds__(TP_THREADS, NJ == 1 ? 3 : 1) attention_tree_pl
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int r = row_of + 4 * i, first = firsts[r];
+      bool hidden = false;
       s[i] += t[i];
       if (j0 + TP_KEYS > past || j0 < first) {        // (what is cached and inside the window is seen)
         const uint32_t view = (uint32_t)tree_view(masks[r], first, past, kv_len, j0);
-        if (!((view >> key) & 1u)) s[i] = -INFINITY;
+        hidden = !((view >> key) & 1u);
+        if (hidden) s[i] = -INFINITY;
       }
       float top = s[i];
 #pragma unroll
       for (int o = 1; o < TP_WARP_KEYS; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
       const float m_new = fmaxf(m[i], top), base = m_new == -INFINITY ? 0.f : m_new;
       const float alpha = exp2f(m[i] - base);
-      s[i] = exp2f(s[i] - base);
+      s[i] = hidden ? -0.f : exp2f(s[i] - base);      // (a key that is not seen is told from one whose weight is too small for a float)
       moved |= m_new > m[i];
       m[i] = m_new;
       l[i] = l[i] * alpha + s[i];
@@ -230,11 +232,11 @@ __global__ void __launch_bounds__(TP_THREADS, NJ == 1 ? 3 : 1) attention_tree_pl
         for (int r = 0; r < TP_TILE; ++r)
 #pragma unroll
           for (int e = 0; e < 4 * NJ; ++e) acc[r][e] = fmaf(p[r], v[e], acc[r][e]);
-      } else {                                        // (a value that a row does not see may be no number)
+      } else {                                        // (one that is no number reaches the rows that see it, however small their weights, and no others)
 #pragma unroll
         for (int r = 0; r < TP_TILE; ++r)
 #pragma unroll
-          for (int e = 0; e < 4 * NJ; ++e) acc[r][e] = p[r] != 0.f ? fmaf(p[r], v[e], acc[r][e]) : acc[r][e];
+          for (int e = 0; e < 4 * NJ; ++e) acc[r][e] = __float_as_uint(p[r]) != 0x80000000u ? fmaf(p[r], v[e], acc[r][e]) : acc[r][e];
       }
     }
     __syncthreads();                                  // the stage may be refilled

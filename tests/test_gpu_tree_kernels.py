@@ -60,6 +60,16 @@ def test_values_that_are_no_numbers(kernel, dtype, dim, parts, nodes):
         check_finite(case, run(case, kernel, parts))
 
 
+@every_kernel
+def test_values_that_are_no_numbers_behind_weights_that_round_to_zero(kernel, dtype, dim, parts):
+    """A weight is never zero in the formula: a row sees such a value however far its score lies below the row's largest."""
+    for what, place in ((math.nan, 70 + 20), (math.inf, 70), (math.nan, 66), (-math.inf, 5)):
+        parents = [-1] + [0] * 39
+        case = Case(dtype, 4, 1, dim, [sees_of(parents)], [70], [depth_of(parents)], seed=place, spread=60.0)
+        spoil(case, 0, place, what, column=3 % dim)
+        check_finite(case, run(case, kernel, parts))
+
+
 @pytest.mark.parametrize("dim, parts", [(64, 1), (128, 1), (128, 4)])
 def test_both_tiles_know_of_values_that_are_no_numbers_in_every_run(dim, parts):
     """Both tiles' warps take the same values out of the shared tile; whoever comes second finds zeros."""
