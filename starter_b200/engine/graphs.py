@@ -209,6 +209,7 @@ class DrawnTokens:
 
     def __init__(self, host=None, done=None, batch=0, ready=None):
         self._host, self._done, self._batch, self._ready = host, done, batch, ready
+        self._read = None     # the device's tokens once the host has them (the list it was given is its own to change)
         #: True if the device also kept these tokens as the sequences' next inputs, so that the next
         #: step can be launched without them
         self.device_feeds = ready is None
@@ -217,7 +218,12 @@ class DrawnTokens:
         if self._ready is None:
             self._done.synchronize()
             self._ready = self._host[:self._batch].tolist()
+            self._read = tuple(self._ready)
         return self._ready
+
+    def was(self, tokens) -> bool:
+        """Whether these are the tokens that the device drew, as far as ``result()`` has been asked (nothing waits here: before that, no)."""
+        return self._read is not None and self._read == tuple(tokens)
 
 
 #: length classes of the captured decode graphs, in cache pages: powers of two and their 1.5-folds

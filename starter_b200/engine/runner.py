@@ -119,6 +119,8 @@ class ModelRunner:
         #: per step: positions, slots, lengths, sampling settings, and the tokens too when the host
         #: has them) instead of going on from what the device holds
         self.self_feeding = True
+        # the last captured step's handle and the temperatures and keys the device draws with
+        self._fed_by = None, None
 
     # ------------------------------------------------------------------ sequences
 
@@ -300,13 +302,23 @@ class ModelRunner:
             if any(t is FED for e in entries for t in e.tokens):
                 raise ValueError("only a captured single-token step can go on from device-held tokens")
             return DrawnTokens(ready=sampler.select(self.step(entries), temperatures, keys, positions))
+        handle, settings = self._fed_by
+        if not any(e.tokens[0] is FED for e in entries):
+            # given tokens and settings count: the device goes on by itself only with the tokens that the host has read from it, as they were drawn
+            given = list(temperatures), list(keys)
+            if handle is None or settings != given or not handle.was([e.tokens[0] for e in entries]):
+                self.graphs.fed, settings = None, given
         self.decode_tokens(entries, temperatures, keys)
-        return self.graphs.fetch(len(entries))
+        handle = self.graphs.fetch(len(entries))
+        self._fed_by = handle, settings
+        return handle
 
     @torch.inference_mode()
     def decode_tokens(self, entries, temperatures, keys) -> torch.Tensor:
-        """Graph path of ``step_and_select``; returns the drawn tokens on the device."""
+        """Graph path of ``step_and_select``; returns the drawn tokens on the device.  Called by itself it goes on from what the device
+        holds for these sequences at these lengths, whatever tokens it is given."""
         cache, graphs = self.cache, self.graphs
+        self._fed_by = None, None
         slots = tuple(e.slot for e in entries)
         for e in entries:
             cache.reserve(e.slot, cache.lengths[e.slot] + 1)
