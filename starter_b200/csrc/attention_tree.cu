@@ -7,7 +7,7 @@
 // references, sums and outputs of their own, which meet at the end.  Everything is float; a result is rounded to the working type
 // once.  Up to eight parts of a sequence's keys are the blocks of one cluster and meet in shared memory.
 //
-// What bounds it: 2 sequences of 13 nodes of 16 heads behind 300 tokens, 256 blocks of two tiles, take 15.4 us: 5 until the first tile is there (the
+// What bounds it: 2 sequences of 13 nodes of 16 heads behind 300 tokens, 256 blocks of two tiles, take 15.6 us: 5 until the first tile is there (the
 // step's arrays, the page's number, the page, which the four blocks of a head's rows all read), 2.9 a tile (the products of queries and
 // keys 1.2, of weights and values 1.1, most of it the shared memory's rate), 3.5 for the meeting of the blocks.  Keys a lane each and
 // rows a warp each read the tile four times over: 17.2; copies and products in turn and a second kernel for the meeting: 33.0.

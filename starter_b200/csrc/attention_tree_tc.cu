@@ -18,7 +18,7 @@
 //
 // What bounds it is the softmax: a step of 128 keys takes 1.07 us with one tile and 1.5 with two, of which the exponentials of 2 x 128 x 128
 // scores are worth 1.07 at 16 a clock and the products 0.55.  16 sequences of 64 nodes behind up to 4,096 tokens each (32 heads of 128 on
-// 8, 128 blocks) take 67 us, 207 MB and 41 GFLOP that are worth 31: the longest sequence's 33 steps, 50 us, behind which the other SMs rest.  Tried
+// 8, 128 blocks) take 65 us, 207 MB and 41 GFLOP that are worth 31: the longest sequence's 33 steps, 50 us, behind which the other SMs rest.  Tried
 // and slower: a cubic in place of every fourth exponential (1.54 us a step) or every second (1.80); sixteen softmax warps, two threads a row (1.78: the
 // weights no longer fit in registers in front of the wait for the product before); both tiles on the same 128 rows where there are no more, every
 // second step each (16 x 32 nodes 57.7 us against 49.7: a copy's way from memory lies in every step).

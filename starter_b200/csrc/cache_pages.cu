@@ -99,7 +99,8 @@ __global__ void __launch_bounds__(CA_THREADS) cache_accept_kernel(const AcceptAr
 //
 // Copies items (cache pages, a slot's state) of several tensors [outer, items, item_bytes]: item source[i] to item target[i], for every
 // outer index.  The pairs travel in the launch's own arguments, so nothing is uploaded.  A block copies one item, 16 bytes a thread at a time.
-// What bounds it is memory: 32 pages of 36 layers (604 MB read and written) take 104 us, 5.8 TB/s; one page of 8 layers 4.4 us, a launch.
+// What bounds it is memory: 32 pages of 36 layers (604 MB read and written) take 103 us, 5.9 TB/s.  With few items it is a block's own way: one page of 8 layers of
+// 4 heads, 16 blocks of 64 KB in 16 rounds of a load and a store each, takes 4.4 us, where the launch and the walk above take 2.7.
 #define CP_MAX_TENSORS 16
 #define CP_MAX_PAIRS 256
 #define CP_THREADS 256

@@ -358,9 +358,9 @@ class ModelRunner:
             if code & 2:
                 problems.append("a row of logits held no finite value")
             if code & 4:
-                problems.append("a wait inside the tensor-core product ran out of time")
+                problems.append("a wait inside a tensor-core product ran out of time")
             if code & 8:
                 problems.append("a wait inside the decode attention kernel ran out of time")
             if code & 16:
-                problems.append("a wait inside the tensor-core prefill attention kernel ran out of time")
+                problems.append("a wait inside the tree attention kernel or the tensor-core prefill attention kernel ran out of time")
             raise RuntimeError("; ".join(problems) or f"device status {code}")
