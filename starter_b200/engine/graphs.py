@@ -225,6 +225,11 @@ class DrawnTokens:
         """Whether these are the tokens that the device drew, as far as ``result()`` has been asked (nothing waits here: before that, no)."""
         return self._read is not None and self._read == tuple(tokens)
 
+    def drawn(self, place: int) -> int:
+        """What the device drew for a place of the batch (waits for it)."""
+        self.result()
+        return self._read[place]
+
 
 #: length classes of the captured decode graphs, in cache pages: powers of two and their 1.5-folds
 HINT_PAGES = tuple(sorted({p for e in range(16) for p in (1 << e, 3 << e >> 1) if p >= 1}))

@@ -302,15 +302,23 @@ class ModelRunner:
             if any(t is FED for e in entries for t in e.tokens):
                 raise ValueError("only a captured single-token step can go on from device-held tokens")
             return DrawnTokens(ready=sampler.select(self.step(entries), temperatures, keys, positions))
+        # given tokens and settings count: the device goes on by itself only with the tokens that the host has read from it, as they were drawn
         handle, settings = self._fed_by
-        if not any(e.tokens[0] is FED for e in entries):
-            # given tokens and settings count: the device goes on by itself only with the tokens that the host has read from it, as they were drawn
-            given = list(temperatures), list(keys)
-            if handle is None or settings != given or not handle.was([e.tokens[0] for e in entries]):
-                self.graphs.fed, settings = None, given
+        given = list(temperatures), list(keys)
+        known = [(i, e.tokens[0]) for i, e in enumerate(entries) if e.tokens[0] is not FED]
+        if len(known) == len(entries):
+            if handle is None or settings != given or not handle.was([t for _, t in known]):
+                self.graphs.fed = None
+        else:
+            slots, lengths = tuple(e.slot for e in entries), [self.cache.lengths[e.slot] for e in entries]
+            if self.graphs.fed == slots and self.graphs.fed_lengths == lengths:      # (if not, the step is refused below)
+                if known and (handle is None or any(handle.drawn(i) != t for i, t in known)):
+                    raise ValueError("a step goes on from device-held tokens for some of its sequences and from others for the rest")
+                if settings != given:
+                    self.graphs.load(slots, None, lengths, temperatures, keys)
         self.decode_tokens(entries, temperatures, keys)
         handle = self.graphs.fetch(len(entries))
-        self._fed_by = handle, settings
+        self._fed_by = handle, given
         return handle
 
     @torch.inference_mode()

@@ -82,3 +82,40 @@ def test_settings_that_change_between_steps(tmp_path_factory):
             out.append(token)
         drawn.append(out)
     assert drawn[0] == drawn[1]
+
+
+def test_settings_that_change_where_the_device_holds_the_tokens(tmp_path_factory):
+    """Steps that go on from the device (FED) at another temperature or key, against steps that are given what was drawn."""
+    runner = runner_for(tmp_path_factory, "A", "float32")
+    sampler, drawn = Sampler(runner.device, runner.status), []
+    for fed in (True, False):
+        slot, token, out = runner.open_sequence(), 5, []
+        for turn, (temperature, key) in enumerate([(0.0, 0), (0.9, 3), (0.9, 3), (2.0, 3), (2.0, 8), (0.0, 8), (1.5, 9)]):
+            token = int(runner.step_and_select([StepEntry(slot, [FED if fed and turn else token], [0])], sampler, [temperature], [key], [turn + 1])[0])
+            out.append(token)
+        drawn.append(out)
+        runner.close_sequence(slot)
+    assert drawn[0] == drawn[1]
+
+
+def test_some_tokens_given_and_some_held(tmp_path_factory):
+    folder, cfg, w = model_case(tmp_path_factory, "A")
+    runner = runner_for(tmp_path_factory, "A", "float32")
+    sampler, vocab = Sampler(runner.device, runner.status), cfg["vocab_size"]
+    texts = [random_prompt(n, vocab, n) for n in (9, 33)]
+    slots = [runner.open_sequence() for _ in texts]
+    runner.step([StepEntry(s, t[:-1]) for s, t in zip(slots, texts)])
+    args = sampler, [0.0] * 2, [0] * 2, [0] * 2
+    first = runner.start_step([StepEntry(s, [t[-1]], [0]) for s, t in zip(slots, texts)], *args)
+    want = [best(cfg, w, t) for t in texts]
+    held = list(runner.cache.lengths)
+    with pytest.raises(ValueError, match="device-held"):
+        runner.start_step([StepEntry(slots[0], [FED], [0]), StepEntry(slots[1], [(want[1] + 1) % vocab], [0])], *args)
+    assert runner.cache.lengths == held and first.result() == want
+    first.result()[1] = -5                               # (the list is the caller's to change)
+    # the drawn one given back is the one that is held
+    second = runner.start_step([StepEntry(slots[0], [FED], [0]), StepEntry(slots[1], [want[1]], [0])], *args)
+    assert second.result() == [best(cfg, w, t + [x]) for t, x in zip(texts, want)]
+    for s in slots:
+        runner.close_sequence(s)
+    runner.check_status()
